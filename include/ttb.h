@@ -48,6 +48,7 @@ extern "C" {
 #define TTB_BFLOAT8_B 3
 #define TTB_BFLOAT4_B 4
 #define TTB_UINT16 6
+#define TTB_FLOAT8_E4M3 16 /* row-major only; not a type of the reference */
 
 /* ---- fused activation after bias (ttnn.linear's `activation`, ttnn/ttnn/operations/matmul.py:59-63) */
 #define TTB_ACT_NONE 0
@@ -77,6 +78,8 @@ extern "C" {
                             the gated MLP's silu(x w1) * (x w3) (models/demos/mistral7b/tt/mistral_mlp.py:51-73,
                             llama2_70b/tt/llama_mlp_optimized.py:165-197) formed inside the launch; out[1] is not written.
                             Workspace: ttb_matmul_gated_workspace_bytes. Row counts of 32, 96, 160 or 224. */
+
+#define TTB_MM_BIAS_ROW_MAJOR 512 /* ttb_linear_float8: the bias is [N] bfloat16 instead of the first row of a tiled [32, N] */
 
 const char *ttb_last_error(void);
 int32_t ttb_version(void);
@@ -225,6 +228,49 @@ int64_t ttb_matmul_decode_static_scratch_bytes(int32_t w_dtype, int64_t batch, i
 int32_t ttb_matmul_decode_static(const void *a_dev, int32_t a_dtype, const void *w_dev, int32_t w_dtype, const void *bias_dev,
                                  void *out_dev, int32_t out_dtype, int64_t batch, int64_t M, int64_t K, int64_t N,
                                  int32_t activation, int32_t flags, void *stream);
+
+/* ---- float8 matmul, expert routing, the experts' MLP ------------------------------------------------
+ * float8 numbers are e4m3 (largest value 448, no infinities): value = code * scale, one fp32 scale for a block of 128 values
+ * of a row or of 128 x 128. These entry points have no counterpart in the reference, whose 8-bit weights are bfloat8_b.
+ *
+ * ttb_quantize_float8: src [outer, H, W] (TTB_FLOAT32 or TTB_BFLOAT16, tiled or row-major) -> codes row-major [outer, H, W], one byte
+ * each, and scales [outer, ceil(H / block_rows), ceil(W / 128)], block_rows 1 or 128:
+ *   scale = max(largest magnitude of the block, 2^-100) / 448, code = x / scale, both quotients rounded to fp32 and the code then to the nearest
+ * e4m3 number, ties to even. A NaN becomes the NaN code and does not count for the scale; a block with an infinity gets the scale inf. */
+int32_t ttb_quantize_float8(const void *src_dev, int32_t src_dtype, int32_t src_row_major, void *codes_dev, void *scales_dev, int64_t outer, int64_t H,
+                            int64_t W, int32_t block_rows, void *stream);
+/* out[rows, N] = act( q(a)[rows, K] x w^T + bias ), fp32 accumulation: `a` (bfloat16) is quantised with block_rows 1; w_codes [N, K] and w_scales
+ * [ceil(N / 128), ceil(K / 128)] as ttb_quantize_float8 leaves them with block_rows 128 (any positive scales serve). K is a multiple of 16, rows and N are
+ * free; tiled tensors have a multiple of 32 rows, and their columns behind N come out as zeros. `bias`: NULL, or bfloat16, the first row of a tiled [32, N]
+ * (TTB_MM_BIAS_ROW_MAJOR: [N]). `out`: TTB_BFLOAT16 or TTB_FLOAT32. Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR, TTB_MM_BIAS_ROW_MAJOR. The workspace
+ * needs no particular contents; it is touched between launch and completion on `stream`. Results repeat bit for bit. */
+int64_t ttb_linear_float8_workspace_bytes(int64_t rows, int64_t K, int64_t N);
+int32_t ttb_linear_float8(const void *a_dev, const void *w_codes_dev, const void *w_scales_dev, const void *bias_dev, void *out_dev, int32_t out_dtype,
+                          int64_t rows, int64_t K, int64_t N, int32_t activation, int32_t flags, void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+#define TTB_SCORE_SOFTMAX 0
+#define TTB_SCORE_SIGMOID 1
+#define TTB_GROUP_MAX 0      /* a group counts as much as its best expert */
+#define TTB_GROUP_TOP2_SUM 1 /* ... as its two best together (the one, where a mask leaves no second) */
+/* Router: for each of outer * H rows of `logits` [outer, H, E] (float32 or bfloat16, tiled or TTB_MM_A_ROW_MAJOR) the k experts of highest choice value and
+ * their weights, row-major [outer * H, k]: experts (uint32) and weights (float32), best first, ties to the lowest index.
+ *   score = softmax or sigmoid of the logits; choice value = score + bias[e] (float32 [E]; NULL: the score); with groups > 1 only the top_groups groups of
+ *   neighbouring experts count. weight = score * scale, divided by the sum of the chosen scores under `renormalize` (zero where that sum is zero).
+ * Order and ties are those of 64-bit choice values. An expert with logit or bias -inf is never chosen; where too few are left, the remaining places hold
+ * the index E and the weight 0. An expert with a NaN is never chosen, and a row with a NaN logit has NaN weights.
+ * E up to 1024, k up to 32, up to 32 groups. */
+int32_t ttb_route_to_experts(const void *logits_dev, int32_t logits_dtype, const void *bias_dev, void *weights_dev, void *experts_dev, int64_t outer, int64_t H,
+                             int64_t E, int32_t k, int32_t score, int32_t groups, int32_t top_groups, int32_t group_score, int32_t renormalize, float scale,
+                             int32_t flags, void *stream);
+/* out[t] = sum_j weights[t, j] * ( q(act(q(x[t]) x gate_e^T) * (q(x[t]) x up_e^T)) x down_e^T ), e = experts[t, j], for the outer * H rows of x [outer, H, hidden]
+ * (bfloat16); an index outside [0, experts) contributes nothing. gate, up: codes [experts, ffn, hidden], down: [experts, hidden, ffn], scales per block of
+ * 128 x 128 as above; q quantises with block_rows 1. hidden and ffn are multiples of 16; out is bfloat16 [outer, H, hidden] (rows and columns that only pad a
+ * tiled result are zero). Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR. Workspace as ttb_linear_float8. Results repeat bit for bit. */
+int64_t ttb_experts_mlp_float8_workspace_bytes(int64_t rows, int64_t experts, int64_t k, int64_t hidden, int64_t ffn);
+int32_t ttb_experts_mlp_float8(const void *x_dev, const void *experts_dev, const void *weights_dev, const void *gate_codes_dev, const void *gate_scales_dev,
+                               const void *up_codes_dev, const void *up_scales_dev, const void *down_codes_dev, const void *down_scales_dev, void *out_dev,
+                               int64_t outer, int64_t H, int64_t experts, int32_t k, int64_t hidden, int64_t ffn, int32_t activation, int32_t flags,
+                               void *workspace_dev, int64_t workspace_bytes, void *stream);
 
 /* Reads (and clears) the device-side status word that kernels with bounded waits set when a wait
  * ran out. Synchronises `stream`. Returns TTB_OK or TTB_E_TIMEOUT. After TTB_E_TIMEOUT the matmul that gave up has

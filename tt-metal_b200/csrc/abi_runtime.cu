@@ -155,6 +155,7 @@ int64_t ttb_buffer_bytes(int32_t dtype, int64_t outer, int64_t Hp, int64_t Wp) {
         case TTB_UINT16: return n * 2;
         case TTB_FLOAT32:
         case TTB_UINT32: return n * 4;
+        case TTB_FLOAT8_E4M3: return n;
         case TTB_BFLOAT8_B: return n / 1024 * ttb::kBfp8TileBytes;
         case TTB_BFLOAT4_B: return n / 1024 * ttb::kBfp4TileBytes;
         default: return -1;

@@ -1,0 +1,384 @@
+// Mixture of experts: the router (scores, groups, top-k, weights) and the experts' gated MLP on float8 weights.
+//
+// Router. A warp takes a row. An expert's choice value is its logit where that orders the scores (no bias, no sum over a group), else score + bias in
+// 64 bits: two experts next to the border may differ by less than 32 bits show, and the choice is a whole number. Ties go to the lowest index.
+//
+// The MLP y[t] = sum_j p[t, j] * down_e( q(act(gate_e x) * (up_e x)) ), e = ids[t, j], runs as
+//   plan      every assignment (t, j) gets a row, sorted by expert and then by t * k + j, with no room between the experts (the matmul's row tiles start at
+//             a multiple of eight rows and leave the rows before an expert's first alone);
+//   quantise  each token once, written to its k rows in the operand layout;
+//   gated     matmul of both weights, product and quantisation in the epilogue;
+//   down      matmul, fp32 rows;
+//   combine   the weighted sum of a token's rows, in the order of j.
+// Sums, weights and the rows between down and combine are fp32; no atomics on numbers, so results repeat bit for bit.
+#include "epilogue.cuh"
+#include "matmul_float8.cuh"
+#include "sm100_ptx.cuh"
+
+#include <math_constants.h>
+
+namespace ttb {
+namespace {
+
+using namespace ptx;
+
+constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
+constexpr int kRouteWarps = 4;
+
+struct RouteArgs {
+    const void *logits;
+    const float *bias;     // [E] or null
+    float *weights;
+    int32_t *experts;
+    int64_t rows, H;
+    int E, k, groups, top_groups;
+    bool bf16, row_major, sigmoid, sum_of_two, renormalize;
+    float scale;
+};
+
+__device__ __forceinline__ void best_of_warp(double &v, int &i) {   // the largest value, the lowest index among equals
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+        const double w = __shfl_xor_sync(0xffffffffu, v, d);
+        const int j = __shfl_xor_sync(0xffffffffu, i, d);
+        if (w > v || (w == v && j < i)) { v = w; i = j; }
+    }
+}
+
+// V: logits per lane.
+template <int V>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs p) {
+    extern __shared__ double choice_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t r = (int64_t)blockIdx.x * kRouteWarps + warp;
+    if (r >= p.rows) return;
+    const int64_t o = r / p.H, h = r - o * p.H;
+    const double none = -CUDART_INF;
+    float x[V];
+    bool nan = false;
+    float most = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = i * 32 + lane;
+        x[i] = -CUDART_INF_F;
+        if (e < p.E) {
+            const int64_t at = p.row_major ? r * p.E + e : o * (((p.H + 31) & ~(int64_t)31) * ((p.E + 31) & ~31)) + tiled_offset(h, e, (p.E + 31) >> 5);
+            x[i] = p.bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p.logits)[at] << 16) : reinterpret_cast<const float *>(p.logits)[at];
+            nan |= x[i] != x[i];
+            most = fmaxf(most, x[i]);
+        }
+    }
+    nan = __any_sync(0xffffffffu, nan);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    // the softmax's denominator, where scores are needed (not for the shares among the chosen ones)
+    const bool by_score = p.bias != nullptr || (p.groups > 1 && p.sum_of_two);
+    double total = 1.0;
+    if (!p.sigmoid && (by_score || !p.renormalize)) {
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i * 32 + lane < p.E && x[i] > -CUDART_INF_F) total += exp((double)x[i] - (double)most);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    }
+    auto score = [&](float v) { return p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)most) / total; };
+    double key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = i * 32 + lane;
+        key[i] = none;
+        if (e < p.E && x[i] > -CUDART_INF_F) {   // (false for a NaN)
+            key[i] = by_score ? score(x[i]) + (p.bias ? (double)p.bias[e] : 0.0) : (double)x[i];
+            if (key[i] != key[i]) key[i] = none;
+        }
+    }
+    if (p.groups > 1) {
+        double *mine = choice_smem + (size_t)warp * p.E;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i * 32 + lane < p.E) mine[i * 32 + lane] = key[i];
+        __syncwarp();
+        const int size = p.E / p.groups;
+        double v = none;
+        if (lane < p.groups) {
+            double second = none;
+            for (int i = 0; i < size; ++i) {
+                const double c = mine[lane * size + i];
+                if (c > v) { second = v; v = c; }
+                else if (c > second) second = c;
+            }
+            if (p.sum_of_two && second > none) v += second;
+        }
+        uint32_t kept = 0;
+        for (int g = 0; g < p.top_groups; ++g) {
+            double b = v;
+            int i = (lane < p.groups && !(kept >> lane & 1)) ? lane : 64;
+            if (i == 64) b = none;
+            best_of_warp(b, i);
+            if (i < 32) kept |= 1u << i;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = i * 32 + lane;
+            if (e < p.E && !(kept >> (e / size) & 1)) key[i] = none;
+        }
+    }
+    // the k best, one after the other; lane j keeps the j-th
+    int my_id = p.E;
+    float my_x = 0.0f;
+    double first = 0.0;   // the largest logit among the chosen
+    for (int j = 0; j < p.k; ++j) {
+        double b = none;
+        int id = kMaxExperts;
+        float bx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (key[i] > b) { b = key[i]; id = i * 32 + lane; bx = x[i]; }
+        const int own = id;
+        best_of_warp(b, id);
+        if (id == kMaxExperts) break;   // nothing is left
+        bx = __shfl_sync(0xffffffffu, bx, id & 31);
+        if (own == id) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i * 32 + lane == id) key[i] = none;
+        }
+        if (lane == j) { my_id = id; my_x = bx; }
+        first = j == 0 ? (double)bx : fmax(first, (double)bx);
+    }
+    double w = 0.0;
+    if (my_id < p.E) w = !p.sigmoid && p.renormalize && !by_score ? exp((double)my_x - first) : score(my_x);
+    if (p.renormalize) {
+        double sum = w;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (sum != 0.0) w /= sum;
+    }
+    if (lane < p.k) {
+        p.experts[r * p.k + lane] = my_id;
+        p.weights[r * p.k + lane] = my_id < p.E ? (nan ? CUDART_NAN_F : (float)(w * (double)p.scale)) : 0.0f;
+    }
+}
+
+// Block e: the rows of expert e. ids outside [0, E) get no row.
+__global__ void __launch_bounds__(256) plan_kernel(const int32_t *ids, int64_t assignments, int E, int32_t *offsets, int32_t *pos) {
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ int warp_sum[8];
+    __shared__ int base_word;
+    const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // rows of the experts before this one
+    int below = 0;
+    for (int64_t i = threadIdx.x; i < assignments; i += 256) {
+        const int x = ids[i];
+        below += x >= 0 && x < e;
+        if (e == 0 && (x < 0 || x >= E)) pos[i] = -1;
+    }
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0) warp_sum[warp] = below;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int s = 0;
+        for (int w = 0; w < 8; ++w) s += warp_sum[w];
+        base_word = s;
+        offsets[e] = s;
+    }
+    __syncthreads();
+    int next = base_word;
+    for (int64_t i0 = 0; i0 < assignments; i0 += 256) {
+        const int64_t i = i0 + threadIdx.x;
+        const bool mine = i < assignments && ids[i] == e;
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) warp_sum[warp] = __popc(votes);
+        __syncthreads();
+        int before = next;
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) before += warp_sum[w];
+            next += warp_sum[w];
+        }
+        if (mine) pos[i] = before + __popc(votes & ((1u << lane) - 1));
+        __syncthreads();
+    }
+    if (e == E - 1 && threadIdx.x == 0) offsets[E] = next;
+}
+
+// out[t] = sum_j weights[t, j] * y[pos[t, j]], four columns a thread; rows that only pad a tile are zero.
+__global__ void __launch_bounds__(256) combine_kernel(const float *y, const int32_t *pos, const float *weights, uint16_t *out, int64_t outer, int64_t H, int64_t Hp,
+                                                      int64_t hidden, int64_t width, int k, bool row_major) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t quads = width / 4, total = outer * Hp * quads;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t pr = i / quads, c = (i - pr * quads) * 4, o = pr / Hp, h = pr - o * Hp;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (h < H && c < hidden) {
+            const int64_t r = o * H + h;
+            for (int j = 0; j < k; ++j) {
+                const int32_t at = pos[r * k + j];
+                if (at < 0) continue;
+                const float w = weights[r * k + j];
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(y + (int64_t)at * hidden + c));
+                s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+            }
+        }
+        uint16_t *dst = out + (row_major ? pr * width + c : o * Hp * width + tiled_offset(h, c, width >> 5));
+        *reinterpret_cast<uint2 *>(dst) = make_uint2((uint32_t)f32_to_bf16_bits(s.x) | ((uint32_t)f32_to_bf16_bits(s.y) << 16),
+                                                     (uint32_t)f32_to_bf16_bits(s.z) | ((uint32_t)f32_to_bf16_bits(s.w) << 16));
+    }
+}
+
+template <typename... P, typename... A>
+int32_t launch_dependent(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, const char *name, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    TTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    TTB_LAUNCH_CHECK(name);
+    return TTB_OK;
+}
+
+template <int V>
+int32_t launch_route(const RouteArgs &p, cudaStream_t stream) {
+    const int64_t blocks = (p.rows + kRouteWarps - 1) / kRouteWarps;
+    const size_t smem = p.groups > 1 ? (size_t)kRouteWarps * p.E * 8 : 0;
+    route_kernel<V><<<(unsigned)blocks, 32 * kRouteWarps, smem, stream>>>(p);
+    TTB_LAUNCH_CHECK("route");
+    return TTB_OK;
+}
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+bool misaligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// Scratch of the experts' MLP.
+struct Scratch {
+    int64_t assignments;
+    int32_t *offsets, *pos;
+    F8Activation x, h;
+    float *y;
+    int64_t bytes;
+};
+F8Activation place(uint8_t *base, int64_t &at, int64_t rows, int64_t cols) {
+    F8Activation a;
+    a.rows_padded = f8_rows_padded(rows);
+    a.scale_pitch = f8_scale_pitch(cols);
+    a.codes = base + at;
+    at = up(at + a.rows_padded * f8_blocks(cols) * kF8Block, 1024);
+    a.scales = reinterpret_cast<float *>(base + at);
+    at = up(at + a.rows_padded * a.scale_pitch * 4, 1024);
+    return a;
+}
+Scratch lay_out(uint8_t *base, int64_t rows, int64_t experts, int64_t k, int64_t hidden, int64_t ffn) {
+    Scratch s;
+    s.assignments = rows * k;
+    int64_t at = 0;
+    s.offsets = reinterpret_cast<int32_t *>(base + at);
+    at = up(at + 4 * (experts + 1), 1024);
+    s.pos = reinterpret_cast<int32_t *>(base + at);
+    at = up(at + 4 * s.assignments, 1024);
+    s.x = place(base, at, s.assignments, hidden);
+    s.h = place(base, at, s.assignments, ffn);
+    s.y = reinterpret_cast<float *>(base + at);
+    at = up(at + s.assignments * hidden * 4, 1024);
+    s.bytes = at;
+    return s;
+}
+constexpr int64_t kMaxExtent = int64_t(1) << 24;
+bool in_range(int64_t v) { return v > 0 && v <= kMaxExtent; }
+
+}  // namespace
+}  // namespace ttb
+
+using ttb::fail;
+
+extern "C" {
+
+int32_t ttb_route_to_experts(const void *logits, int32_t logits_dtype, const void *bias, void *weights, void *experts, int64_t outer, int64_t H, int64_t E,
+                             int32_t k, int32_t score, int32_t groups, int32_t top_groups, int32_t group_score, int32_t renormalize, float scale, int32_t flags,
+                             void *stream) {
+    const char *who = "ttb_route_to_experts";
+    if (!logits || !weights || !experts) return fail(TTB_E_INVALID, "%s: null tensor pointer", who);
+    if (logits_dtype != TTB_FLOAT32 && logits_dtype != TTB_BFLOAT16) return fail(TTB_E_UNSUPPORTED, "%s: the logits must be float32 or bfloat16", who);
+    if (flags & ~TTB_MM_A_ROW_MAJOR) return fail(TTB_E_INVALID, "%s: unknown flags %d", who, flags);
+    if (outer <= 0 || H <= 0 || outer > INT32_MAX || H > INT32_MAX || outer * H > INT32_MAX) return fail(TTB_E_INVALID, "%s: the row count must be between 1 and 2^31 - 1", who);
+    if (E < 1 || E > ttb::kMaxExperts) return fail(TTB_E_UNSUPPORTED, "%s: between 1 and %d experts, got %lld", who, ttb::kMaxExperts, (long long)E);
+    if (k < 1 || k > ttb::kMaxTopK || k > E) return fail(TTB_E_INVALID, "%s: k must be between 1 and the number of experts, at most %d, got %d", who, ttb::kMaxTopK, k);
+    if (score != TTB_SCORE_SOFTMAX && score != TTB_SCORE_SIGMOID) return fail(TTB_E_INVALID, "%s: unknown score %d", who, score);
+    if (groups < 1 || groups > ttb::kMaxGroups || E % groups) return fail(TTB_E_INVALID, "%s: the experts must divide into 1 to %d groups of one size", who, ttb::kMaxGroups);
+    if (top_groups < 1 || top_groups > groups) return fail(TTB_E_INVALID, "%s: top_groups must be between 1 and the number of groups", who);
+    if (k > E / groups * top_groups) return fail(TTB_E_INVALID, "%s: %d groups of %lld experts have no %d to choose", who, top_groups, (long long)(E / groups), k);
+    if (group_score != TTB_GROUP_MAX && group_score != TTB_GROUP_TOP2_SUM) return fail(TTB_E_INVALID, "%s: unknown group score %d", who, group_score);
+    if (ttb::misaligned(logits, logits_dtype == TTB_FLOAT32 ? 4 : 2) || (bias && ttb::misaligned(bias, 4)) || ttb::misaligned(weights, 4) || ttb::misaligned(experts, 4))
+        return fail(TTB_E_INVALID, "%s: misaligned tensor", who);
+    ttb::RouteArgs p;
+    p.logits = logits; p.bias = (const float *)bias; p.weights = (float *)weights; p.experts = (int32_t *)experts;
+    p.rows = outer * H; p.H = H; p.E = (int)E; p.k = k; p.groups = groups; p.top_groups = top_groups;
+    p.bf16 = logits_dtype == TTB_BFLOAT16; p.row_major = flags & TTB_MM_A_ROW_MAJOR; p.sigmoid = score == TTB_SCORE_SIGMOID;
+    p.sum_of_two = group_score == TTB_GROUP_TOP2_SUM; p.renormalize = renormalize != 0; p.scale = scale;
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (E <= 32) return ttb::launch_route<1>(p, s);
+    if (E <= 64) return ttb::launch_route<2>(p, s);
+    if (E <= 128) return ttb::launch_route<4>(p, s);
+    if (E <= 256) return ttb::launch_route<8>(p, s);
+    return ttb::launch_route<32>(p, s);
+}
+
+int64_t ttb_experts_mlp_float8_workspace_bytes(int64_t rows, int64_t experts, int64_t k, int64_t hidden, int64_t ffn) {
+    using ttb::in_range;
+    if (!in_range(rows) || experts < 1 || experts > ttb::kMaxExperts || k < 1 || k > ttb::kMaxTopK || !in_range(rows * k) || !in_range(hidden) || !in_range(ffn)) return -1;
+    return ttb::lay_out(nullptr, rows, experts, k, hidden, ffn).bytes;
+}
+
+int32_t ttb_experts_mlp_float8(const void *x, const void *ids, const void *weights, const void *gate_codes, const void *gate_scales, const void *up_codes,
+                               const void *up_scales, const void *down_codes, const void *down_scales, void *out, int64_t outer, int64_t H, int64_t experts,
+                               int32_t k, int64_t hidden, int64_t ffn, int32_t activation, int32_t flags, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *who = "ttb_experts_mlp_float8";
+    if (!x || !ids || !weights || !gate_codes || !gate_scales || !up_codes || !up_scales || !down_codes || !down_scales || !out)
+        return fail(TTB_E_INVALID, "%s: null tensor pointer", who);
+    if (flags & ~(TTB_MM_A_ROW_MAJOR | TTB_MM_OUT_ROW_MAJOR)) return fail(TTB_E_INVALID, "%s: unknown flags %d", who, flags);
+    if (activation < TTB_ACT_NONE || activation > TTB_ACT_SILU) return fail(TTB_E_INVALID, "%s: unknown activation %d", who, activation);
+    if (!ttb::in_range(outer) || !ttb::in_range(H)) return fail(TTB_E_INVALID, "%s: rows must be between 1 and 2^24", who);
+    const int64_t rows = outer * H, need = ttb_experts_mlp_float8_workspace_bytes(rows, experts, k, hidden, ffn);
+    if (need < 0)
+        return fail(TTB_E_INVALID, "%s: between 1 and 2^24 rows times k, hidden and ffn sizes of at most 2^24, 1 to %d experts and k of 1 to %d", who, ttb::kMaxExperts, ttb::kMaxTopK);
+    if (hidden % 16 || ffn % 16) return fail(TTB_E_INVALID, "%s: the hidden and ffn sizes must be multiples of 16 (got %lld, %lld)", who, (long long)hidden, (long long)ffn);
+    for (const void *p : {x, gate_codes, up_codes, down_codes, (const void *)out})
+        if (ttb::misaligned(p, 16)) return fail(TTB_E_INVALID, "%s: activations, codes and the result must be 16-byte aligned", who);
+    for (const void *p : {ids, weights, gate_scales, up_scales, down_scales})
+        if (ttb::misaligned(p, 4)) return fail(TTB_E_INVALID, "%s: misaligned tensor", who);
+    if (!ttb::workspace_serves(workspace, workspace_bytes, need)) return fail(TTB_E_WORKSPACE, "%s: needs %lld bytes of 256-byte aligned workspace", who, (long long)need);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const bool x_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;
+    const ttb::Scratch w = ttb::lay_out(static_cast<uint8_t *>(workspace), rows, experts, k, hidden, ffn);
+    if (int32_t rc = ttb::launch_dependent(ttb::plan_kernel, (unsigned)experts, 256, s, "plan", (const int32_t *)ids, w.assignments, (int)experts, w.offsets, w.pos)) return rc;
+    if (int32_t rc = ttb::launch_quantize_operand(x, x_rm, outer, H, hidden, w.x, w.pos, k, nullptr, 0, s)) return rc;
+    ttb::F8Matmul m = {};
+    m.a = w.x;
+    m.w[0] = {gate_codes, (const float *)gate_scales};
+    m.w[1] = {up_codes, (const float *)up_scales};
+    m.rows = w.assignments; m.K = hidden; m.N = ffn;
+    m.experts = (int)experts; m.offsets = w.offsets;
+    m.act = activation;
+    m.gated = true; m.h = w.h;
+    if (int32_t rc = ttb::launch_matmul_float8(m, s)) return rc;
+    ttb::F8Matmul d = {};
+    d.a = w.h;
+    d.w[0] = {down_codes, (const float *)down_scales};
+    d.rows = w.assignments; d.K = ffn; d.N = hidden;
+    d.experts = (int)experts; d.offsets = w.offsets;
+    d.act = TTB_ACT_NONE;
+    d.out = w.y; d.out_dtype = TTB_FLOAT32; d.out_row_major = true;
+    if (int32_t rc = ttb::launch_matmul_float8(d, s)) return rc;
+    const int64_t Hp = out_rm ? H : ttb::round_up32(H), width = out_rm ? hidden : ttb::round_up32(hidden);
+    const int64_t want = (outer * Hp * (width / 4) + 255) / 256;
+    return ttb::launch_dependent(ttb::combine_kernel, (unsigned)(want < 148 * 32 ? want : 148 * 32), 256, s, "combine", (const float *)w.y, (const int32_t *)w.pos,
+                                 (const float *)weights, (uint16_t *)out, outer, H, Hp, hidden, width, (int)k, out_rm);
+}
+
+}  // extern "C"

@@ -633,7 +633,7 @@ int32_t make_weight_maps(const DecodeArgs &p, int fmt, WeightMaps &maps, int gro
     return TTB_OK;
 }
 
-static int32_t tensor_map_encoder(void **out) {
+int32_t tensor_map_encoder(void **out) {
     static void *encode = nullptr;
     if (!encode) {
         void *fn = nullptr;

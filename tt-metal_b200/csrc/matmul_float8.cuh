@@ -1,0 +1,44 @@
+// What the float8 matmul, its quantiser and the experts' MLP share.
+#pragma once
+#include "float8.cuh"
+
+namespace ttb {
+
+// Quantised activations in scratch (layout: float8.cuh).
+struct F8Activation {
+    uint8_t *codes;      // [blocks of 128 columns][rows_padded][128]
+    float *scales;       // [rows_padded][scale_pitch]
+    int64_t rows_padded;
+    int64_t scale_pitch;
+};
+
+struct F8Weight {
+    const void *codes;   // [experts, N, K], row-major
+    const float *scales; // [experts, ceil(N / 128), ceil(K / 128)]
+};
+
+// act(x w^T + bias) of all rows with one weight, or of runs of rows with an expert's weight each.
+struct F8Matmul {
+    F8Activation a;
+    F8Weight w[2];           // the second: the up projection of a gated pair
+    int64_t rows, K, N;
+    int experts;             // 0: one weight for all rows
+    const int32_t *offsets;  // [experts + 1], device: rows offsets[e] .. offsets[e + 1] - 1 are expert e's
+    int act;
+    // either a plain result
+    void *out;
+    int out_dtype;
+    bool out_row_major;
+    const uint16_t *bias;    // bfloat16 [N], or the first row of a tiled [32, N]; may be null
+    bool bias_row_major;
+    // or act(x w0^T) * (x w1^T), quantised again
+    bool gated;
+    F8Activation h;
+};
+int32_t launch_matmul_float8(const F8Matmul &p, cudaStream_t stream);
+
+// Quantises [outer, H, K] bfloat16 rows into `out`: row r to row r, or (pos) to the rows pos[r * k + j] >= 0. Also clears zero[0 .. zeros - 1].
+int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, int64_t H, int64_t K, const F8Activation &out, const int32_t *pos, int k,
+                                int32_t *zero, int zeros, cudaStream_t stream);
+
+}  // namespace ttb

@@ -6,6 +6,7 @@
 #include <pybind11/stl.h>
 
 #include "ccl.hpp"
+#include "float8.hpp"
 #include "ops.hpp"
 
 namespace py = pybind11;
@@ -16,7 +17,8 @@ PYBIND11_MODULE(_ttnn, m) {
 
     py::enum_<DataType>(m, "DataType")
         .value("BFLOAT16", DataType::BFLOAT16).value("FLOAT32", DataType::FLOAT32).value("UINT32", DataType::UINT32)
-        .value("BFLOAT8_B", DataType::BFLOAT8_B).value("BFLOAT4_B", DataType::BFLOAT4_B).value("UINT16", DataType::UINT16);
+        .value("BFLOAT8_B", DataType::BFLOAT8_B).value("BFLOAT4_B", DataType::BFLOAT4_B).value("UINT16", DataType::UINT16)
+        .value("FLOAT8_E4M3", DataType::FLOAT8_E4M3);
     py::enum_<Layout>(m, "Layout").value("ROW_MAJOR", Layout::ROW_MAJOR).value("TILE", Layout::TILE);
     py::enum_<StorageType>(m, "StorageType")
         .value("OWNED", StorageType::OWNED).value("DEVICE", StorageType::DEVICE).value("BORROWED", StorageType::BORROWED)
@@ -203,6 +205,31 @@ PYBIND11_MODULE(_ttnn, m) {
           py::arg("gather_first") = false, py::arg("wait_slot") = -1, py::arg("gated") = false);
     m.def("nvtx_push", [](const std::string &name) { ttb_nvtx_push(name.c_str()); });
     m.def("nvtx_pop", []() { ttb_nvtx_pop(); });
+    // ---- float8 and mixture of experts -----------------------------------------------------------------------------
+    m.def("quantize_float8",
+          [](const Tensor &t, int block_rows) {
+              const Float8 q = quantize_float8(t, block_rows);
+              return py::make_tuple(q.codes, q.scales);
+          },
+          py::arg("tensor"), py::arg("block_rows"));
+    m.def("linear_float8",
+          [](const Tensor &x, const Tensor &codes, const Tensor &scales, const std::optional<Tensor> &bias, std::optional<DataType> dtype,
+             const std::optional<std::string> &activation) { return linear_float8(x, {codes, scales}, bias, dtype, activation); },
+          py::arg("input_tensor"), py::arg("codes"), py::arg("scales"), py::kw_only(), py::arg("bias") = std::nullopt, py::arg("dtype") = std::nullopt,
+          py::arg("activation") = std::nullopt);
+    m.def("route_to_experts",
+          [](const Tensor &logits, int k, const std::string &score, const std::optional<Tensor> &bias, int groups, int top_groups, const std::string &group_score,
+             bool renormalize, float scale) {
+              const Routing r = route_to_experts(logits, k, score, bias, groups, top_groups, group_score, renormalize, scale);
+              return py::make_tuple(r.weights, r.experts);
+          },
+          py::arg("logits"), py::arg("k"), py::kw_only(), py::arg("score"), py::arg("bias") = std::nullopt, py::arg("groups"), py::arg("top_groups"),
+          py::arg("group_score"), py::arg("renormalize"), py::arg("scale"));
+    m.def("experts_mlp_float8",
+          [](const Tensor &x, const Tensor &experts, const Tensor &weights, const Tensor &gate_codes, const Tensor &gate_scales, const Tensor &up_codes,
+             const Tensor &up_scales, const Tensor &down_codes, const Tensor &down_scales, const std::optional<std::string> &activation) {
+              return experts_mlp_float8(x, experts, weights, {gate_codes, gate_scales}, {up_codes, up_scales}, {down_codes, down_scales}, activation);
+          });
     m.def("mul", &multiply, py::arg("input_tensor_a"), py::arg("input_tensor_b"));
     m.def("matmul", &matmul, py::arg("input_tensor_a"), py::arg("input_tensor_b"), py::kw_only(), py::arg("dtype") = std::nullopt,
           py::arg("program_config") = std::nullopt);

@@ -56,6 +56,8 @@ Tensor from_host_buffer(const void *src, const std::vector<int64_t> &dims, DataT
         if (layout != Layout::TILE) throw_error("ttnn.from_torch: bfloat8_b/bfloat4_b requires TILE_LAYOUT!");
         if (src_dtype != DataType::FLOAT32 && src_dtype != DataType::BFLOAT16)
             throw_error("ttnn.from_torch: block-float tensors are packed from float32 or bfloat16 data");
+    } else if (dtype == DataType::FLOAT8_E4M3 && layout != Layout::ROW_MAJOR) {
+        throw_error("ttnn.from_torch: float8_e4m3 requires ROW_MAJOR_LAYOUT!");
     } else if (src_dtype != dtype) {
         throw_error("ttnn.from_torch: the host data must already have the requested element type");
     }
@@ -129,6 +131,7 @@ void to_host_buffer(const Tensor &t, void *dst) {
 Tensor to_layout(const Tensor &t, Layout layout) {
     if (layout != Layout::ROW_MAJOR && layout != Layout::TILE) throw_error("ttnn.to_layout: Unsupported layout!");
     if (t.layout() == layout) return t;
+    if (t.dtype() == DataType::FLOAT8_E4M3) throw_error("ttnn.to_layout: float8_e4m3 tensors are row-major");
     const bool on_device = t.storage_type() == StorageType::DEVICE;
     Tensor d = on_device ? t : to_device_storage(t, current_or_default_device());
     Device *dev = d.device();
@@ -276,6 +279,7 @@ Tensor pad(const Tensor &t, const std::vector<int64_t> &output_shape, const std:
     const char *op = "Tensor.pad";
     if (!t.is_allocated()) throw_error(std::string(op) + ": the tensor has been deallocated");
     if (t.layout() != Layout::ROW_MAJOR) throw_error(std::string(op) + ": Tensor layout must be ROW_MAJOR for padding");
+    if (t.dtype() == DataType::FLOAT8_E4M3) throw_error(std::string(op) + ": float8_e4m3 tensors are not supported");
     const std::vector<int64_t> in = as4(t.shape().padded(), 1, op), out = as4(output_shape, 1, op), st = as4(input_start, 0, op);
     for (int i = 0; i < 4; ++i)
         if (st[i] < 0 || in[i] + st[i] > out[i]) throw_error(std::string(op) + ": the input tensor does not fit the output shape at the given start");
@@ -304,6 +308,7 @@ Tensor unpad(const Tensor &t, const std::vector<int64_t> &start, const std::vect
     const char *op = "Tensor.unpad";
     if (!t.is_allocated()) throw_error(std::string(op) + ": the tensor has been deallocated");
     if (t.layout() != Layout::ROW_MAJOR) throw_error(std::string(op) + ": Tensor layout must be ROW_MAJOR for unpadding");
+    if (t.dtype() == DataType::FLOAT8_E4M3) throw_error(std::string(op) + ": float8_e4m3 tensors are not supported");
     const std::vector<int64_t> in = as4(t.shape().padded(), 1, op), st = as4(start, 0, op), en = as4(end, 0, op);
     std::vector<int64_t> out(4);
     for (int i = 0; i < 4; ++i) {

@@ -18,6 +18,7 @@ int element_size(DataType d) {
         case DataType::UINT16: return 2;
         case DataType::FLOAT32:
         case DataType::UINT32: return 4;
+        case DataType::FLOAT8_E4M3: return 1;
         default: throw_error("element_size: block-float and invalid data types have no per-element size");
     }
 }
@@ -30,6 +31,7 @@ const char *to_string(DataType d) {
         case DataType::BFLOAT8_B: return "DataType.BFLOAT8_B";
         case DataType::BFLOAT4_B: return "DataType.BFLOAT4_B";
         case DataType::UINT16: return "DataType.UINT16";
+        case DataType::FLOAT8_E4M3: return "DataType.FLOAT8_E4M3";
         default: return "DataType.INVALID";
     }
 }

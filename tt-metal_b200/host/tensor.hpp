@@ -18,7 +18,8 @@
 namespace ttnn_b200 {
 
 // Numeric values follow tt::tt_metal::DataType / Layout (tt_eager/tensor/types.hpp:24-34).
-enum class DataType : int { BFLOAT16 = 0, FLOAT32 = 1, UINT32 = 2, BFLOAT8_B = 3, BFLOAT4_B = 4, UINT16 = 6, INVALID = 7 };
+enum class DataType : int { BFLOAT16 = 0, FLOAT32 = 1, UINT32 = 2, BFLOAT8_B = 3, BFLOAT4_B = 4, UINT16 = 6, INVALID = 7,
+                            FLOAT8_E4M3 = 16 /* not a type of the reference; row-major only */ };
 enum class Layout : int { ROW_MAJOR = 0, TILE = 1, INVALID = 2 };
 enum class StorageType : int { OWNED = 0, DEVICE = 1, BORROWED = 2, MULTI_DEVICE = 3, MULTI_DEVICE_HOST = 4 };
 enum class BufferType : int { DRAM = 0, L1 = 1 };

@@ -20,7 +20,7 @@ if TTNN_ENABLE_LOGGING:
 
 from .types import *  # noqa: F401,F403
 from .types import (DataType, Layout, StorageType, Shape, Tensor, Device, CoreGrid, MemoryConfig, MathFidelity, DeviceGrid,
-                    bfloat16, bfloat8_b, bfloat4_b, float32, uint16, uint32, TILE_LAYOUT, ROW_MAJOR_LAYOUT, TILE_SIZE,
+                    bfloat16, bfloat8_b, bfloat4_b, float32, uint16, uint32, float8_e4m3, TILE_LAYOUT, ROW_MAJOR_LAYOUT, TILE_SIZE,
                     DRAM_MEMORY_CONFIG, L1_MEMORY_CONFIG, WormholeComputeKernelConfig, GrayskullComputeKernelConfig,
                     DeviceComputeKernelConfig)
 from .device import open_device, close_device, manage_device, synchronize_device
@@ -31,6 +31,7 @@ from .operations.core import (from_torch, to_torch, to_layout, to_device, from_d
                               load_tensor, as_tensor, is_tensor_storage_on_device)
 from .operations.matmul import (matmul, linear, mul, MatmulProgramConfig, MatmulDefaultProgramConfig, MatmulMultiCoreReuseProgramConfig,
                                 MatmulMultiCoreReuseMultiCastProgramConfig, MatmulMultiCoreReuseMultiCast1DProgramConfig)
+from .operations.float8 import Float8Tensor, quantize_float8, linear_float8, route_to_experts, experts_mlp_float8
 from .operations.ccl import all_gather, linear_all_gather, linear_gated, linear_multi, wait_for_gather
 
 from . import decorators
@@ -38,7 +39,8 @@ from .decorators import register_operation, register_pre_operation_hook, registe
 
 # every public operation goes through the per-operation wrapper (logging, hooks, NVTX) unless fast runtime mode is on
 for _name in ("from_torch", "to_torch", "to_layout", "to_device", "from_device", "reshape", "as_tensor", "dump_tensor", "load_tensor",
-              "matmul", "linear", "mul", "all_gather", "linear_all_gather", "linear_gated", "linear_multi"):
+              "matmul", "linear", "mul", "all_gather", "linear_all_gather", "linear_gated", "linear_multi", "quantize_float8", "linear_float8",
+              "route_to_experts", "experts_mlp_float8"):
     globals()[_name] = register_operation("ttnn." + _name)(globals()[_name])
 del _name
 

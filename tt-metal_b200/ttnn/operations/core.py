@@ -17,8 +17,10 @@ from .. import _ttnn
 from .. import types as T
 from ..multi_device import MultiDeviceTensor, TensorToMesh, MeshToTensor
 
-_TORCH_TO_TTNN = {torch.bfloat16: T.bfloat16, torch.float32: T.float32, torch.int32: T.uint32, torch.int16: T.uint16}
-_TTNN_TO_TORCH = {T.bfloat16: torch.bfloat16, T.float32: torch.float32, T.uint32: torch.int32, T.uint16: torch.int16}
+_TORCH_TO_TTNN = {torch.bfloat16: T.bfloat16, torch.float32: T.float32, torch.int32: T.uint32, torch.int16: T.uint16,
+                  torch.float8_e4m3fn: T.float8_e4m3}
+_TTNN_TO_TORCH = {T.bfloat16: torch.bfloat16, T.float32: torch.float32, T.uint32: torch.int32, T.uint16: torch.int16,
+                  T.float8_e4m3: torch.float8_e4m3fn}
 
 
 def _is_block_float(dtype):

@@ -11,6 +11,7 @@ float32 = DataType.FLOAT32
 bfloat16 = DataType.BFLOAT16
 bfloat8_b = DataType.BFLOAT8_B
 bfloat4_b = DataType.BFLOAT4_B
+float8_e4m3 = DataType.FLOAT8_E4M3      # not a type of the reference: row-major codes, see quantize_float8
 
 BufferType = _ttnn.BufferType
 TensorMemoryLayout = _ttnn.TensorMemoryLayout
