@@ -242,8 +242,9 @@ int32_t ttb_quantize_float8(const void *src_dev, int32_t src_dtype, int32_t src_
 /* out[rows, N] = act( q(a)[rows, K] x w^T + bias ), fp32 accumulation: `a` (bfloat16) is quantised with block_rows 1; w_codes [N, K] and w_scales
  * [ceil(N / 128), ceil(K / 128)] as ttb_quantize_float8 leaves them with block_rows 128 (any positive scales serve). K is a multiple of 16, rows and N are
  * free; tiled tensors have a multiple of 32 rows, and their columns behind N come out as zeros. `bias`: NULL, or bfloat16, the first row of a tiled [32, N]
- * (TTB_MM_BIAS_ROW_MAJOR: [N]). `out`: TTB_BFLOAT16 or TTB_FLOAT32. Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR, TTB_MM_BIAS_ROW_MAJOR. The workspace
- * needs no particular contents; it is touched between launch and completion on `stream`. Results repeat bit for bit. */
+ * (TTB_MM_BIAS_ROW_MAJOR: [N]). `out`: TTB_BFLOAT16 or TTB_FLOAT32. Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR, TTB_MM_BIAS_ROW_MAJOR and, as for ttb_matmul,
+ * with whose calls a workspace can be shared, TTB_MM_WORKSPACE_ZEROED (else the counters at its head are cleared with a memset) and TTB_MM_WEIGHTS_RESIDENT. The
+ * workspace is touched between launch and completion on `stream`. Results repeat bit for bit. */
 int64_t ttb_linear_float8_workspace_bytes(int64_t rows, int64_t K, int64_t N);
 int32_t ttb_linear_float8(const void *a_dev, const void *w_codes_dev, const void *w_scales_dev, const void *bias_dev, void *out_dev, int32_t out_dtype,
                           int64_t rows, int64_t K, int64_t N, int32_t activation, int32_t flags, void *workspace_dev, int64_t workspace_bytes, void *stream);
@@ -265,7 +266,7 @@ int32_t ttb_route_to_experts(const void *logits_dev, int32_t logits_dtype, const
 /* out[t] = sum_j weights[t, j] * ( q(act(q(x[t]) x gate_e^T) * (q(x[t]) x up_e^T)) x down_e^T ), e = experts[t, j], for the outer * H rows of x [outer, H, hidden]
  * (bfloat16); an index outside [0, experts) contributes nothing. gate, up: codes [experts, ffn, hidden], down: [experts, hidden, ffn], scales per block of
  * 128 x 128 as above; q quantises with block_rows 1. hidden and ffn are multiples of 16; out is bfloat16 [outer, H, hidden] (rows and columns that only pad a
- * tiled result are zero). Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR. Workspace as ttb_linear_float8. Results repeat bit for bit. */
+ * tiled result are zero). Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR. The workspace needs no particular contents. Results repeat bit for bit. */
 int64_t ttb_experts_mlp_float8_workspace_bytes(int64_t rows, int64_t experts, int64_t k, int64_t hidden, int64_t ffn);
 int32_t ttb_experts_mlp_float8(const void *x_dev, const void *experts_dev, const void *weights_dev, const void *gate_codes_dev, const void *gate_scales_dev,
                                const void *up_codes_dev, const void *up_scales_dev, const void *down_codes_dev, const void *down_scales_dev, void *out_dev,

@@ -161,13 +161,15 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
     }
 }
 
-// Block e: the rows of expert e. ids outside [0, E) get no row.
-__global__ void __launch_bounds__(256) plan_kernel(const int32_t *ids, int64_t assignments, int E, int32_t *offsets, int32_t *pos) {
+// Block e: the rows of expert e. ids outside [0, E) get no row. row_of: the row of the activations (of a tiled tensor: with its padding) that a row is from.
+__global__ void __launch_bounds__(256) plan_kernel(const int32_t *ids, int64_t assignments, int E, int k, int H, int Hp, int32_t *offsets, int32_t *pos, int32_t *row_of, int32_t *zero,
+                                                   int zeros) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ int warp_sum[8];
     __shared__ int base_word;
     const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = e * 256 + threadIdx.x; i < zeros; i += gridDim.x * 256) zero[i] = 0;
     // rows of the experts before this one
     int below = 0;
     for (int64_t i = threadIdx.x; i < assignments; i += 256) {
@@ -197,7 +199,11 @@ __global__ void __launch_bounds__(256) plan_kernel(const int32_t *ids, int64_t a
             if (w < warp) before += warp_sum[w];
             next += warp_sum[w];
         }
-        if (mine) pos[i] = before + __popc(votes & ((1u << lane) - 1));
+        if (mine) {
+            const int at = before + __popc(votes & ((1u << lane) - 1)), row = (int)(i / k);
+            pos[i] = at;
+            row_of[at] = row / H * Hp + row % H;
+        }
         __syncthreads();
     }
     if (e == E - 1 && threadIdx.x == 0) offsets[E] = next;
@@ -215,10 +221,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const float *y, const int3
         if (h < H && c < hidden) {
             const int64_t r = o * H + h;
             for (int j = 0; j < k; ++j) {
-                const int32_t at = pos[r * k + j];
+                const int32_t at = __ldcg(pos + r * k + j);
                 if (at < 0) continue;
                 const float w = weights[r * k + j];
-                const float4 v = __ldcs(reinterpret_cast<const float4 *>(y + (int64_t)at * hidden + c));
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(y + (int64_t)at * hidden + c));
                 s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
             }
         }
@@ -259,9 +265,11 @@ bool misaligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintp
 // Scratch of the experts' MLP.
 struct Scratch {
     int64_t assignments;
-    int32_t *offsets, *pos;
+    int32_t *offsets, *pos, *row_of;
     F8Activation x, h;
     float *y;
+    int32_t *gated_tickets, *down_tickets;   // neighbours, cleared together
+    float *partials;                         // of either matmul, one after the other
     int64_t bytes;
 };
 F8Activation place(uint8_t *base, int64_t &at, int64_t rows, int64_t cols) {
@@ -282,10 +290,17 @@ Scratch lay_out(uint8_t *base, int64_t rows, int64_t experts, int64_t k, int64_t
     at = up(at + 4 * (experts + 1), 1024);
     s.pos = reinterpret_cast<int32_t *>(base + at);
     at = up(at + 4 * s.assignments, 1024);
-    s.x = place(base, at, s.assignments, hidden);
+    s.row_of = reinterpret_cast<int32_t *>(base + at);
+    at = up(at + 4 * s.assignments, 1024);
+    s.x = f8_quantises_itself(s.assignments, experts) ? F8Activation{} : place(base, at, s.assignments, hidden);
     s.h = place(base, at, s.assignments, ffn);
     s.y = reinterpret_cast<float *>(base + at);
     at = up(at + s.assignments * hidden * 4, 1024);
+    s.gated_tickets = reinterpret_cast<int32_t *>(base + at);
+    s.down_tickets = reinterpret_cast<int32_t *>(base + at + kF8TicketBytes);
+    at += 2 * kF8TicketBytes;
+    s.partials = reinterpret_cast<float *>(base + at);
+    at += f8_partial_bytes(s.assignments, true);
     s.bytes = at;
     return s;
 }
@@ -356,23 +371,33 @@ int32_t ttb_experts_mlp_float8(const void *x, const void *ids, const void *weigh
     const cudaStream_t s = (cudaStream_t)stream;
     const bool x_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;
     const ttb::Scratch w = ttb::lay_out(static_cast<uint8_t *>(workspace), rows, experts, k, hidden, ffn);
-    if (int32_t rc = ttb::launch_dependent(ttb::plan_kernel, (unsigned)experts, 256, s, "plan", (const int32_t *)ids, w.assignments, (int)experts, w.offsets, w.pos)) return rc;
-    if (int32_t rc = ttb::launch_quantize_operand(x, x_rm, outer, H, hidden, w.x, w.pos, k, nullptr, 0, s)) return rc;
+    if (int32_t rc = ttb::launch_dependent(ttb::plan_kernel, (unsigned)experts, 256, s, "plan", (const int32_t *)ids, w.assignments, (int)experts, (int)k, (int)H,
+                                           (int)(x_rm ? H : ttb::round_up32(H)), w.offsets, w.pos, w.row_of, w.gated_tickets, (int)(2 * ttb::kF8TicketBytes / 4)))
+        return rc;
     ttb::F8Matmul m = {};
-    m.a = w.x;
+    if (ttb::f8_quantises_itself(w.assignments, experts)) {
+        m.x = {static_cast<const uint16_t *>(x), w.row_of, x_rm ? hidden : (hidden + 31) / 32 * 1024, !x_rm};
+    } else {
+        if (int32_t rc = ttb::launch_quantize_operand(x, x_rm, outer, H, hidden, w.x, w.pos, k, false, s)) return rc;
+        m.a = w.x;
+        m.early = true;   // (the quantiser waits for the plan before it lets the matmul start)
+    }
     m.w[0] = {gate_codes, (const float *)gate_scales};
     m.w[1] = {up_codes, (const float *)up_scales};
     m.rows = w.assignments; m.K = hidden; m.N = ffn;
     m.experts = (int)experts; m.offsets = w.offsets;
     m.act = activation;
     m.gated = true; m.h = w.h;
+    m.tickets = w.gated_tickets; m.partials = w.partials;
     if (int32_t rc = ttb::launch_matmul_float8(m, s)) return rc;
     ttb::F8Matmul d = {};
     d.a = w.h;
+    d.early = true;   // (so does the gated matmul)
     d.w[0] = {down_codes, (const float *)down_scales};
     d.rows = w.assignments; d.K = ffn; d.N = hidden;
     d.experts = (int)experts; d.offsets = w.offsets;
     d.act = TTB_ACT_NONE;
+    d.tickets = w.down_tickets; d.partials = w.partials;
     d.out = w.y; d.out_dtype = TTB_FLOAT32; d.out_row_major = true;
     if (int32_t rc = ttb::launch_matmul_float8(d, s)) return rc;
     const int64_t Hp = out_rm ? H : ttb::round_up32(H), width = out_rm ? hidden : ttb::round_up32(hidden);

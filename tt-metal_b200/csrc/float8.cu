@@ -24,10 +24,10 @@ __device__ __forceinline__ void load8(const Source &s, int64_t o, int64_t row, i
     const T *p = reinterpret_cast<const T *>(s.ptr) + o * s.slab + (s.tiled ? tiled_offset(row, c, s.pitch) : row * s.pitch + c);
     if (s.vector && c + 8 <= W) {
         if (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p)), b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+            const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(p));
             const uint32_t h[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -128,10 +128,10 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(Source src, uint8_
 
 // Activations into the operand layout. Without `pos` row r goes to row r; with it to the rows pos[r * k + j] (-1: nowhere).
 __global__ void __launch_bounds__(256) quantize_operand_kernel(Source src, int64_t rows, int64_t H, int64_t K, F8Activation out, const int32_t *pos, int k,
-                                                               int32_t *zero, int zeros) {
+                                                               bool early) {
+    if (early) ptx::grid_dep_launch();
     ptx::grid_dep_wait();
-    ptx::grid_dep_launch();
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < zeros; i += gridDim.x * 256) zero[i] = 0;
+    if (!early) ptx::grid_dep_launch();
     const int64_t blocks = f8_blocks(K);
     const int sub = threadIdx.x & 15;
     const int64_t total = rows * blocks, step = (int64_t)gridDim.x * 16;
@@ -166,7 +166,7 @@ Source make_source(const void *ptr, int dtype, bool row_major, int64_t H, int64_
 }  // namespace
 
 int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, int64_t H, int64_t K, const F8Activation &out, const int32_t *pos, int k,
-                                int32_t *zero, int zeros, cudaStream_t stream) {
+                                bool early, cudaStream_t stream) {
     const int64_t rows = outer * H, want = (rows * f8_blocks(K) + 15) / 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(want < 148 * 8 ? (want > 0 ? want : 1) : 148 * 8));
@@ -177,7 +177,7 @@ int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, in
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, quantize_operand_kernel, make_source(a, TTB_BFLOAT16, row_major, H, K), rows, H, K, out, pos, k, zero, zeros));
+    TTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, quantize_operand_kernel, make_source(a, TTB_BFLOAT16, row_major, H, K), rows, H, K, out, pos, k, early));
     TTB_LAUNCH_CHECK("quantize_operand");
     return TTB_OK;
 }

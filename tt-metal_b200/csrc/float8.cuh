@@ -28,6 +28,12 @@ __device__ __forceinline__ uint2 f8_pack8(const float (&v)[8], float scale) {
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
+__device__ __forceinline__ uint32_t f8_pack4(const float (&v)[4], float scale) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[0], scale), __fdiv_rn(v[1], scale)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2], scale), __fdiv_rn(v[3], scale)), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+
 // Quantised activations in scratch: for every block of 128 columns all rows, 128 bytes each, with the 16-byte chunks of a row
 // exchanged as the MMA's 128-byte-swizzled K-major operand wants them (chunk ^= row % 8), so that any run of rows that starts at a
 // multiple of eight is one contiguous copy. Byte of (row, block, column-in-block):

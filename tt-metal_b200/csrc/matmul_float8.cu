@@ -5,98 +5,30 @@
 // A tile is 128 rows x W blocks of 128 weight rows (output columns). Per block of 128 K values
 //   * one warp fetches the operands: the weight's 128 x 128 bytes straight from the row-major tensor with a 128-byte-swizzled tensor map, the rows'
 //     codes with one contiguous copy (they are kept in the operand layout, float8.cuh);
-//   * one warp issues four tcgen05.mma (kind::f8f6f4, 128 x 128 W x 32) into one of two tensor memory accumulators;
-//   * eight warps add the finished accumulator, times the two scales, to fp32 sums in registers while the MMAs fill the other. A thread holds one row
+//   * one of two warps issues four tcgen05.mma (kind::f8f6f4, 128 x 128 W x 32) into one of 4 / W tensor memory accumulators (waits, four MMAs and a commit
+//     take an issuing thread some 650 clocks, a block's MMAs 256 W);
+//   * eight warps add the finished accumulator, times the two scales, to fp32 sums in registers while the MMAs fill the others. A thread holds one row
 //     and 64 W columns, so the scales are one number a block and thread.
 // The tensor cores' own chain of additions is thus 128 products long whatever K is.
+// Blocks take whole tiles round by round; the tiles left after the last whole round form one list of (tile, K block) units, which is dealt out evenly.
+// The blocks that share a tile leave their fp32 sums in scratch and take a ticket; the last one adds them in block order (so results
+// repeat bit for bit) and finishes the rows. No block waits for another. A block's range ends with the first part of a tile, whose other parts are the
+// beginnings of other blocks' ranges: it mostly finds them all there and adds them to its sums in registers.
 // Every mbarrier wait is bounded; a wait that runs out raises a status word instead of hanging.
-#include <cuda.h>
-
-#include "epilogue.cuh"
-#include "matmul_float8.cuh"
-#include "sm100_ptx.cuh"
+#include "float8_tiles.cuh"
 
 namespace ttb {
 unsigned barrier_limit_kcycles();
 int32_t status_word_address(int **out);
 int32_t tensor_map_encoder(void **out);
+int stream_blocks();
+int32_t launch_matmul_float8_few(const f8::Args &p, int act, int W, int R, bool gated, int grid, int smem, int dev, cudaStream_t stream);
 namespace {
 
+using namespace f8;
 using namespace ptx;
 
 constexpr int BM = 128;
-constexpr int kMaxStages = 12;
-constexpr int kEpiWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kThreads = 32 * 10;
-constexpr int kSmemLimit = 232448 - 1024;   // the rest: static shared memory
-constexpr int kMaxExperts = 1024;
-
-struct alignas(64) Args {
-    CUtensorMap wmap[2];
-    const float *sw[2];
-    F8Activation a, h;
-    const int32_t *offsets;
-    const uint16_t *bias;
-    void *out;
-    int64_t N;
-    int rows, experts, Kb, Nb, ct;   // ct: column tiles
-    int a_rows, stages, stage_bytes; // rows of a stage's activations (a multiple of 8); the ring
-    int act, out_dtype, out_row_major, bias_row_major, out_aligned;   // out_aligned: bytes that a store may have
-    unsigned wait_limit;
-    int *status;
-};
-
-__device__ __forceinline__ long long wait_clocks(const Args &p) { return (long long)p.wait_limit << 10; }
-
-// K-major operand with the 128-byte swizzle: rows of 128 bytes, eight rows form a 1024-byte atom in which 16-byte chunk c of row r lies at c ^ r.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// Instruction descriptor for kind::f8f6f4, both operands e4m3 and K-major, fp32 accumulator.
-__host__ __device__ constexpr uint32_t instr_desc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-
-__device__ __forceinline__ void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-        "}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-
-// A tile of the launch: rows [lo, hi) of expert e, kept as rows base .. base + 127 (base: a multiple of eight, at most lo), column tile c.
-struct Tile {
-    int e, lo, hi, base, c;
-};
-
-__device__ __forceinline__ int row_tiles(int lo, int hi) { return hi > lo ? (hi - (lo & ~7) + BM - 1) / BM : 0; }
-
-// Tile t of the launch. Row tiles vary fastest (up to 16 of them), so that blocks that run together share weights.
-__device__ __forceinline__ Tile tile_of(const Args &p, const int *off, const int *cum, int t) {
-    Tile s;
-    int lo = 0, hi = p.rows;
-    s.e = 0;
-    if (p.experts) {
-        int a = 0, b = p.experts;   // the last expert with cum[e] <= t
-        while (b - a > 1) {
-            const int m = (a + b) >> 1;
-            if (cum[m] <= t) a = m; else b = m;
-        }
-        s.e = a;
-        t -= cum[a];
-        lo = off[a];
-        hi = off[a + 1];
-    }
-    const int rt = row_tiles(lo, hi), per = 16 * p.ct;
-    const int group = t / per, in = t - group * per, height = min(16, rt - group * 16);
-    const int r = group * 16 + in % height;
-    s.c = in / height;
-    s.base = (lo & ~7) + r * BM;
-    s.lo = max(lo, s.base);
-    s.hi = min(hi, s.base + BM);
-    return s;
-}
 
 // 16 columns from n on of one row.
 __device__ __forceinline__ void store16(const Args &p, int64_t row, int64_t n, const float *v) {
@@ -129,43 +61,51 @@ __device__ __forceinline__ void store16(const Args &p, int64_t row, int64_t n, c
     }
 }
 
+// 16 columns from n on: bias, activation, store.
+template <int ACT>
+__device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, float *v) {
+    if (p.bias && n < p.N) {
+        const uint16_t *b = p.bias + (p.bias_row_major ? n : tiled_offset(0, n, p.N >> 5));   // (16 columns of the first tile row are neighbours)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (n + j < p.N) v[j] += __uint_as_float((uint32_t)__ldg(b + j) << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = apply_activation_t<ACT>(v[j]);
+    store16(p, row, n, v);
+}
+
+// A thread's columns of a whole tile. With an activation 16 at a time in a loop that shifts the sums down: 128 inlined activations are up to 60 KB of code, which
+// runs cold once a tile (a 350 x 4544 x 4672 launch with gelu: 39 us against 21 without finishing its tiles).
 template <int ACT, int NC>
 __device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n0, float (&acc)[NC]) {
+    if constexpr (ACT == TTB_ACT_NONE) {
 #pragma unroll
-    for (int q = 0; q < NC; q += 16) {
-        float v[16];
+        for (int q = 0; q < NC; q += 16) finish16<ACT>(p, row, n0 + q, acc + q);
+    } else {
+#pragma unroll 1
+        for (int q = 0; q < NC; q += 16) {
+            finish16<ACT>(p, row, n0 + q, acc);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int64_t n = n0 + q + j;
-            float b = 0.0f;
-            if (p.bias && n < p.N) b = p.bias_row_major ? __uint_as_float((uint32_t)__ldg(p.bias + n) << 16) : bias_at(p.bias, n);
-            v[j] = apply_activation_t<ACT>(acc[q + j] + b);
+            for (int j = 0; j + 16 < NC; ++j) acc[j] = acc[j + 16];
         }
-        store16(p, row, n0 + q, v);
-        asm volatile("" ::: "memory");   // (keeps the compiler from fetching all groups' bias values at once)
     }
 }
 
-// act(g) * u of one row's 64 columns, quantised with the scale of all 128: the warp with the other 64 exchanges its largest magnitudes through `red` (a
-// barrier of the two warps, in bounded waits like every other). Returns false where that ran out.
+// act(g) * u of one row's 64 columns from part * 64 on, quantised with the scale of all 128: the two warps of the rows exchange their largest magnitudes
+// through `red`.
 template <int ACT>
-__device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid, int c, int half, int lane_row, float (&acc)[128], float (*red)[BM], uint32_t bar,
-                                             volatile int *abort_flag) {
+__device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid, int c, int part, int lane_row, float (&acc)[128], float (*red)[BM], Meeting &meet) {
     float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < 64; ++j) {
         acc[j] = apply_activation_t<ACT>(acc[j]) * acc[64 + j];
         m = fmaxf(m, fabsf(acc[j]));
     }
-    auto meet = [&](uint32_t parity) {
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, 55, wait_clocks(p)));
-    };
-    red[half][lane_row] = m;
-    if (!meet(0)) return false;
-    const float scale = f8_scale(fmaxf(m, red[half ^ 1][lane_row]));
-    if (!meet(1)) return false;   // (the next tile writes `red` again)
+    red[part][lane_row] = m;
+    if (!meet(p)) return false;
+    const float scale = f8_scale(fmaxf(m, red[part ^ 1][lane_row]));
+    if (!meet(p)) return false;   // (the next tile writes `red` again)
     if (!valid) return true;
 #pragma unroll
     for (int q = 0; q < 64; q += 16) {
@@ -176,22 +116,43 @@ __device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid,
             u[j] = acc[q + 8 + j];
         }
         const uint2 x = f8_pack8(v, scale), y = f8_pack8(u, scale);
-        *reinterpret_cast<uint4 *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, half * 64 + q)) = make_uint4(x.x, x.y, y.x, y.y);
+        *reinterpret_cast<uint4 *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, part * 64 + q)) = make_uint4(x.x, x.y, y.x, y.y);
     }
-    if (half == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
+    if (part == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
     return true;
 }
 
+// 32 bytes, one sector.
+__device__ __forceinline__ void load_partial8(const float *src, float (&v)[8]) {
+    asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void store_partial8(float *dst, const float *v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+
+// Eight warps add up, with 64 W columns a thread. (Sixteen with half as many were no faster: 2048 x 8192 x 28672 523 us against 556.)
+constexpr int kAddWarps = 8, kFetchWarp = kAddWarps, kIssueWarp = kFetchWarp + 1, kHandWarp = kIssueWarp + kIssuers, kManyThreads = 32 * (kHandWarp + 1);
+// Registers a thread: of the 384 x 168 that the block is launched with, the adding warps of the two-block tiles take 216 each (128 sums, 32 values on their way
+// from tensor memory) and leave 72 to the other four.
+constexpr int kRegs = 168, kAddRegs = 216, kOtherRegs = 72;
+static_assert(kAddWarps * kAddRegs + 4 * kOtherRegs == (kAddWarps + 4) * kRegs, "a warpgroup that asks for more than the block holds waits for good");
+
 // W: weight blocks per tile. GATED: the two blocks are the same rows of the two weights.
-template <int W, bool GATED>
-__global__ void __launch_bounds__(kThreads, 1) matmul_float8_kernel(const __grid_constant__ Args p) {
+template <int ACT, int W, bool GATED>
+__global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ Args p) {
     static_assert(!GATED || W == 2, "a gated tile takes a block of either weight");
-    constexpr int NC = 64 * W;   // columns of an epilogue thread
+    constexpr int NC = 64 * W;      // columns of an adding thread
+    constexpr int NB = 4 / W;       // accumulators: all of tensor memory
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 6];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 10];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_word;
     __shared__ int tiles_word;
+    __shared__ volatile int ticket;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint8_t *after = smem + p.stages * p.stage_bytes;
@@ -199,155 +160,179 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_float8_kernel(const __grid
     int *off = reinterpret_cast<int *>(after + (GATED ? 2 * BM * 4 : 0));
     int *cum = off + p.experts + 1;
     const uint32_t bar0 = smem_u32(bars);
-    auto full = [&](int s) { return bar0 + 8u * s; };
-    auto done = [&](int s) { return bar0 + 8u * (kMaxStages + s); };   // the MMAs of the stage have read it and its accumulator is complete
-    auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
-    auto pair = [&](int quad) { return bar0 + 8u * (2 * kMaxStages + 2 + quad); };
+    auto pair = [&](int quad) { return bar0 + 8u * (2 * kMaxStages + 4 + quad); };
+    const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + 8), handed_bar = all_bar + 8;
     volatile int *abort_flag = &abort_word;
+    const Ring ring = {sbase, bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(done(s), 1);
+            mbar_init(ring.full(s), 1);
+            mbar_init(ring.done(s), 1);
         }
-        for (int b = 0; b < 2; ++b) mbar_init(acc_empty(b), kEpiWarps);
+        for (int b = 0; b < NB; ++b) mbar_init(ring.acc_empty(b), kAddWarps);
         for (int q = 0; q < 4; ++q) mbar_init(pair(q), 2);
+        mbar_init(all_bar, kAddWarps);
+        mbar_init(handed_bar, kAddWarps);
         abort_word = 0;
         fence_mbar_init();
     }
-    if (warp == kMmaWarp) {
-        tmem_alloc(smem_u32(&tmem_slot), 256 * W);
+    if (warp == kIssueWarp) {
+        tmem_alloc(smem_u32(&tmem_slot), 512);
         tmem_relinquish();
     }
-    grid_dep_wait();
-    grid_dep_launch();
-    if (p.experts) {
-        for (int i = threadIdx.x; i <= p.experts; i += kThreads) off[i] = p.offsets[i];
-        __syncthreads();
-        if (warp == 0) {
-            int run = 0;
-            for (int i = 0; i < p.experts; i += 32) {
-                int x = i + lane < p.experts ? row_tiles(off[i + lane], off[i + lane + 1]) * p.ct : 0, sum = x;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, sum, d);
-                    if (lane >= d) sum += y;
-                }
-                if (i + lane < p.experts) cum[i + lane] = run + sum - x;
-                run += __shfl_sync(0xffffffffu, sum, 31);
-            }
-            if (lane == 0) tiles_word = run;
-        }
-    } else if (threadIdx.x == 0) {
-        tiles_word = row_tiles(0, p.rows) * p.ct;
-    }
+    // The kernel before may still run (programmatic dependency): what is read before grid_dep_wait - the weights and the experts' row ranges - was written
+    // before that kernel let this one start.
+    if (!p.early) grid_dep_wait();
+    count_tiles(p, off, cum, &tiles_word);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = tmem_slot;
-    const int tiles = tiles_word;
+    Walk walk(p, tiles_word);
+    Segment seg;
 
-    if (warp == kProducerWarp) {
-        const bool leader = elect_one();
-        fence_proxy_async_global();   // the activations were written by ordinary stores of the kernel before
-        int s = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const Tile T = tile_of(p, off, cum, t);
-            const uint32_t a_bytes = (uint32_t)(((T.hi + 7) & ~7) - T.base) * kF8Block;
-            for (int kb = 0; kb < p.Kb; ++kb) {
-                if (!__all_sync(0xffffffffu, mbar_wait(done(s), ph ^ 1, abort_flag, p.status, 51, wait_clocks(p)))) { ok = false; break; }
-                if (leader) {
-                    const uint32_t dst = sbase + (uint32_t)(s * p.stage_bytes), w_dst = dst + (uint32_t)(p.a_rows * kF8Block);
-                    mbar_arrive_expect_tx(full(s), a_bytes + W * kF8BlockBytes);
+    if (warp >= kAddWarps) {
+        if (W == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kFetchWarp) {
+            fetch<W, GATED, false, false>(p, ring, walk, off, cum);
+        } else if (warp < kIssueWarp + kIssuers) {
+            issue_mmas<NB>(p, ring, walk, off, cum, warp - kIssueWarp, [&](uint32_t src, int buf, const Tile &) {
+                const uint64_t a = smem_desc_sw128(src), b = smem_desc_sw128(src + (uint32_t)(p.a_rows * kF8Block));
 #pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        tma_load_3d_plain(w_dst + j * kF8BlockBytes, &p.wmap[GATED ? j : 0], kb * kF8Block, (GATED ? T.c : T.c * W + j) * kF8Block, T.e, full(s));
-                    bulk_g2s_plain(dst, p.a.codes + ((int64_t)kb * p.a.rows_padded + T.base) * kF8Block, a_bytes, full(s));
-                }
-                if (++s == p.stages) { s = 0; ph ^= 1; }
-            }
+                for (int k = 0; k < 4; ++k)   // 32 bytes of K further: two 16-byte units in the descriptor's address
+                    mma_e4m3_ss(tmem_base + (uint32_t)(buf * 128 * W), a + 2 * k, b + 2 * k, instr_desc_e4m3(BM, 128 * W), k > 0);
+            });
+        } else {
+            hand_over<ACT, W, GATED>(p, handed_bar, abort_flag, walk, off, cum);
         }
-    } else if (warp == kMmaWarp) {
-        const bool leader = elect_one();
-        constexpr uint32_t idesc = instr_desc_e4m3(BM, 128 * W);
-        int s = 0, n = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x)
-            for (int kb = 0; kb < p.Kb; ++kb, ++n) {
-                const int buf = n & 1;
-                if (!__all_sync(0xffffffffu, mbar_wait(acc_empty(buf), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, p.status, 52, wait_clocks(p))) ||
-                    !__all_sync(0xffffffffu, mbar_wait(full(s), ph, abort_flag, p.status, 53, wait_clocks(p)))) { ok = false; break; }
-                tc_fence_after_sync();
-                if (leader) {
-                    const uint32_t src = sbase + (uint32_t)(s * p.stage_bytes);
-                    const uint64_t a = smem_desc_sw128(src), b = smem_desc_sw128(src + (uint32_t)(p.a_rows * kF8Block));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)   // 32 bytes of K further: two 16-byte units in the descriptor's address
-                        mma_e4m3_ss(tmem_base + (uint32_t)(buf * 128 * W), a + 2 * k, b + 2 * k, idesc, k > 0);
-                    mma_commit(done(s));
-                }
-                if (++s == p.stages) { s = 0; ph ^= 1; }
-            }
     } else {
-        const int quad = warp & 3, half = warp >> 2;
+        if (W == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
+        grid_dep_wait();
+        const int quad = warp & 3, part = warp >> 2;   // 32 rows, half of the columns
         const int lane_row = quad * 32 + lane;
+        // accumulator column of sum j: 64 of either weight (gated), else NC neighbours
+        auto column = [&](int j) { return GATED ? (j / 64) * 128 + part * 64 + (j & 63) : part * NC + j; };
+        Meeting meet = {pair(quad), 0, abort_flag}, meet_all = {all_bar, 0, abort_flag};
         int s = 0, n = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const Tile T = tile_of(p, off, cum, t);
+        while (ok && walk.next(seg)) {
+            const Tile T = tile_of(p, off, cum, seg.tile);
             const int row = T.base + lane_row;
             const bool valid = row >= T.lo && row < T.hi;
-            const bool warp_valid = T.base + quad * 32 < T.hi;
-            const float *sa = p.a.scales + (int64_t)min(row, T.hi - 1) * p.a.scale_pitch;
-            const float *sw0, *sw1;
-            if (GATED) {
-                sw0 = p.sw[0] + ((int64_t)T.e * p.Nb + T.c) * p.Kb;
-                sw1 = p.sw[1] + ((int64_t)T.e * p.Nb + T.c) * p.Kb;
-            } else {
-                sw0 = sw1 = p.sw[0] + ((int64_t)T.e * p.Nb + min(T.c * W + (W == 2 ? half : 0), p.Nb - 1)) * p.Kb;
-            }
-            // columns of the accumulator: 64 of either weight (gated), else NC neighbours
-            const uint32_t col0 = GATED ? half * 64 : half * NC;
+            const bool warp_valid = T.base + quad * 32 < T.hi && T.base + quad * 32 + 32 > T.lo;
+            // scales: of this thread's row four blocks at a time, of the weight (the same for all threads) lane l that of block 32 i + l; both one step ahead
+            const float *const sa = p.a.scales + (int64_t)max(min(row, T.hi - 1), T.lo) * p.a.scale_pitch;
+            const int64_t wrow = GATED ? T.c : min(T.c * W + (W == 2 ? part : 0), p.Nb - 1);
+            const float *const sw0 = p.sw[0] + ((int64_t)T.e * p.Nb + wrow) * p.Kb;
+            const float *const sw1 = GATED ? p.sw[1] + ((int64_t)T.e * p.Nb + wrow) * p.Kb : nullptr;
+            auto load_a = [&](int kb) { return kb < p.a.scale_pitch ? __ldcg(reinterpret_cast<const float4 *>(sa + kb)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+            auto load_w = [&](const float *sw, int kb) { return kb + lane < p.Kb ? __ldg(sw + kb + lane) : 0.0f; };
+            float4 xa = load_a(seg.kb0 & ~3), xa_next = load_a((seg.kb0 & ~3) + 4);
+            float w0 = load_w(sw0, seg.kb0 & ~31), w0_next = load_w(sw0, (seg.kb0 & ~31) + 32);
+            float w1 = GATED ? load_w(sw1, seg.kb0 & ~31) : 0.0f, w1_next = GATED ? load_w(sw1, (seg.kb0 & ~31) + 32) : 0.0f;
             float acc[NC];
 #pragma unroll
             for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
-            for (int kb = 0; kb < p.Kb; ++kb, ++n) {
-                const int buf = n & 1;
-                const float x = __ldcg(sa + kb), f0 = x * __ldg(sw0 + kb), f1 = GATED ? x * __ldg(sw1 + kb) : f0;
-                if (!__all_sync(0xffffffffu, mbar_wait(done(s), ph, abort_flag, p.status, 54, wait_clocks(p)))) { ok = false; break; }
+            for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
+                const int buf = n % NB;
+                const float x = (kb & 2) ? ((kb & 1) ? xa.w : xa.z) : ((kb & 1) ? xa.y : xa.x);
+                const float f0 = x * __shfl_sync(0xffffffffu, w0, kb & 31), f1 = GATED ? x * __shfl_sync(0xffffffffu, w1, kb & 31) : f0;
+                if ((kb & 3) == 3) {
+                    xa = xa_next;
+                    xa_next = load_a(kb + 5);
+                    if ((kb & 31) == 31) {
+                        w0 = w0_next;
+                        w0_next = load_w(sw0, kb + 33);
+                        if (GATED) {
+                            w1 = w1_next;
+                            w1_next = load_w(sw1, kb + 33);
+                        }
+                    }
+                }
+                if (!__all_sync(0xffffffffu, mbar_wait(ring.done(s), ph, abort_flag, p.status, 54, wait_clocks(p)))) { ok = false; break; }
                 tc_fence_after_sync();
                 if (warp_valid) {
                     const uint32_t t0 = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * 128 * W);
 #pragma unroll
-                    for (int q = 0; q < NC; q += 32) {
-                        uint32_t r0[16], r1[16];
-                        const uint32_t c = GATED ? (q / 64) * 128 + half * 64 + (q & 63) : col0 + q;
-                        tmem_ld16(t0 + c, r0);
-                        tmem_ld16(t0 + c + 16, r1);
+                    for (int q = 0; q < NC; q += 64 / W) {
+                        uint32_t r[4 / W][16];
+#pragma unroll
+                        for (int i = 0; i < 4 / W; ++i) tmem_ld16(t0 + column(q + 16 * i), r[i]);
                         tmem_ld_wait();
                         const float f = GATED && q >= 64 ? f1 : f0;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            acc[q + j] = fmaf(__uint_as_float(r0[j]), f, acc[q + j]);
-                            acc[q + 16 + j] = fmaf(__uint_as_float(r1[j]), f, acc[q + 16 + j]);
-                        }
+                        for (int i = 0; i < 4 / W; ++i)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) acc[q + 16 * i + j] = fmaf(__uint_as_float(r[i][j]), f, acc[q + 16 * i + j]);
                     }
                 }
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty(buf));
+                if (lane == 0) mbar_arrive(ring.acc_empty(buf));
                 if (++s == p.stages) { s = 0; ph ^= 1; }
             }
             if (!ok) break;
+            if (seg.kb1 - seg.kb0 < p.Kb) {
+                // ---- a shared tile ----
+                const Sharing sh(walk, seg);
+                const int tile_floats = p.partial_rows * 128 * W, mine = lane_row * (128 * W);
+                const bool last_segment = walk.u >= walk.u_end;
+                bool all_here = false;
+                if ((int)blockIdx.x == sh.c0 && last_segment) {
+                    // The first of the sharers, which comes to this tile at the end of its range: the others mostly have been here long ago.
+                    if (threadIdx.x == 0) ticket = read_tickets(p.tickets + sh.q);
+                    if (!meet_all(p)) break;
+                    all_here = ticket == sh.c1 - sh.c0;
+                    if (!meet_all(p)) break;   // (`ticket` is written again)
+                }
+                if (all_here) {
+                    if (threadIdx.x == 0) p.tickets[sh.q] = 0;
+                    if (valid) {
+#pragma unroll 1
+                        for (int b = sh.c0 + 1; b <= sh.c1; ++b) {
+                            const float *src = sh.part(p, b, tile_floats) + mine;
+#pragma unroll
+                            for (int j = 0; j < NC; j += 32) {
+                                float v[4][8];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) load_partial8(src + column(j + 8 * i), v[i]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) acc[j + 8 * i + e] += v[i][e];
+                            }
+                        }
+                    }
+                } else {
+                    if (valid) {
+                        float *dst = sh.part(p, (int)blockIdx.x, tile_floats) + mine;
+#pragma unroll
+                        for (int j = 0; j < NC; j += 8) store_partial8(dst + column(j), acc + j);
+                    }
+                    if (!last_segment) {   // the hand-over warp sees to the rest while the next segment runs
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(handed_bar);
+                        continue;
+                    }
+                    if (!meet_all(p)) break;
+                    if (threadIdx.x == 0) ticket = take_ticket(p.tickets + sh.q);
+                    if (!meet_all(p)) break;
+                    if (ticket != sh.c1 - sh.c0) continue;
+                    if (threadIdx.x == 0) p.tickets[sh.q] = 0;
+                    // the last one adds them: row after row, each by a whole warp
+                    auto part_of = [&](int block) { return sh.part(p, block, tile_floats); };
+                    const int r_end = T.hi - T.base, r0 = T.lo - T.base + warp;
+                    add_parts<ACT, W, GATED, 4, 2, kAddWarps>(p, part_of, sh.c0, sh.c1, r0, r_end, T.base, T.c, lane);
+                    continue;
+                }
+            }
             if constexpr (GATED) {
-                TTB_DISPATCH_ACT(p.act, ok = finish_gated<ACT>(p, row, valid, T.c, half, lane_row, acc, red, pair(quad), abort_flag));
+                ok = finish_gated<ACT>(p, row, valid, T.c, part, lane_row, acc, red, meet);
             } else {
-                if (valid) TTB_DISPATCH_ACT(p.act, (finish_row<ACT, NC>(p, row, (int64_t)T.c * 128 * W + half * NC, acc)));
+                if (valid) finish_row<ACT, NC>(p, row, (int64_t)T.c * 128 * W + part * NC, acc);
             }
         }
     }
@@ -360,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_float8_kernel(const __grid
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == kMmaWarp) {
+    if (warp == kIssueWarp) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem_base, 256 * W);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
@@ -382,17 +367,17 @@ int32_t make_map(const void *codes, int64_t experts, int64_t N, int64_t K, CUten
     return TTB_OK;
 }
 
-template <int W, bool GATED>
+template <int ACT, int W, bool GATED>
 int32_t launch(const Args &p, int grid, int smem, int dev, cudaStream_t stream) {
     static Once once[64];
     if (int32_t rc = once[dev].run([&]() -> int32_t {
-            TTB_CUDA_TRY(cudaFuncSetAttribute(matmul_float8_kernel<W, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+            TTB_CUDA_TRY(cudaFuncSetAttribute(matmul_float8_kernel<ACT, W, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
             return TTB_OK;
         }))
         return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kManyThreads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -400,12 +385,41 @@ int32_t launch(const Args &p, int grid, int smem, int dev, cudaStream_t stream) 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, matmul_float8_kernel<W, GATED>, p));
+    TTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, matmul_float8_kernel<ACT, W, GATED>, p));
     TTB_LAUNCH_CHECK("matmul_float8");
     return TTB_OK;
 }
 
 }  // namespace
+
+static int partial_rows(int64_t rows) { return rows >= BM - 31 ? BM : (int)(f8_rows_padded(rows) + 31) / 32 * 32; }
+int64_t f8_partial_bytes(int64_t rows, bool gated) { return 2 * (int64_t)stream_blocks() * partial_rows(rows) * 128 * 2 * 4; }
+
+// Rows of a tile, by all rows or by what an expert has on average.
+static int rows_per_tile(int64_t rows, int64_t experts) {
+    const int64_t hit = rows < experts ? rows : experts, mean = experts ? (rows + hit - 1) / hit : rows;
+    return mean <= (experts ? 24 : 32) ? 32 : mean <= (experts ? 56 : 64) ? 64 : BM;
+}
+static int64_t mean_rows(int64_t rows, int64_t experts) {
+    const int64_t hit = rows < experts ? rows : experts;
+    return experts ? (rows + hit - 1) / hit : rows;
+}
+bool f8_quantises_itself(int64_t rows, int64_t experts) { return mean_rows(rows, experts) <= (experts ? 4 : 8); }
+
+// Weight blocks per tile of a plain matmul. Two make the longer unit of work; which is better goes by the whole rounds over the multiprocessors (us, one / two
+// blocks a tile):
+//  * many rows: a round of two-block tiles takes 1.47 times as long as one of one-block tiles. 512 x 8192 x 8192 60.0 / 49.1, 350 x 8192 x 8192 58.5 / 45.9, 2048 x
+//    4096 x 4096 70.0 / 57.4, but 512 x 4096 x 4096 21.1 / 28.5, 1024 x 4544 x 4672 42.2 / 55.0, 2048 x 4544 x 4672 79.5 / 85.1;
+//  * 9 to 64 rows: where one-block tiles are more than a round. 32 x 8192 x 28672 55.1 / 44.7, but 32 x 4544 x 18176 23.1 / 24.0, 32 x 28672 x 8192 49.7 / 51.0;
+//  * up to 8 rows (quantised by the kernel itself, whose warps do that once a tile): from 1000 one-block units on. 1 x 8192 x 28672 46.9 / 40.8, 1 x 4096 x 4096
+//    11.3 / 10.0, but 1 x 8192 x 1024 9.3 / 10.2, 1 x 4096 x 1024 8.4 / 9.0.
+static int weight_blocks(const F8Matmul &m, int R, int64_t sms) {
+    const int64_t hit = m.experts ? (m.rows < m.experts ? m.rows : m.experts) : 1, row_tiles = hit * ((m.rows / hit + R - 1) / R), nb = f8_blocks(m.N);
+    const int64_t one = row_tiles * nb, two = row_tiles * ((nb + 1) / 2);
+    if (m.x.ptr) return one * f8_blocks(m.K) >= 1000 ? 2 : 1;
+    if (R < BM) return one > sms ? 2 : 1;
+    return (two + sms - 1) / sms * 147 < (one + sms - 1) / sms * 100 ? 2 : 1;
+}
 
 int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     Args p;
@@ -418,30 +432,47 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     p.sw[0] = m.w[0].scales;
     p.sw[1] = m.w[1].scales;
     p.a = m.a; p.h = m.h;
+    p.x = m.x; p.K = m.K;
+    p.early = m.early;
+    p.row_mask = m.x.ptr ? 0 : 7;
     p.offsets = m.offsets; p.bias = m.bias; p.out = m.out; p.N = m.N;
     p.rows = (int)m.rows; p.experts = m.experts;
     p.Kb = (int)f8_blocks(m.K); p.Nb = (int)f8_blocks(m.N);
-    const int W = m.gated ? 2 : 1;
+    const int sms = stream_blocks();
+    const int R = rows_per_tile(m.rows, m.experts), W = m.gated ? 2 : weight_blocks(m, R, sms);
+    p.Kb = (int)f8_blocks(m.K);
+    // Where tiles are shared (units a block takes at least; units that sharing has to save): the hand-over costs what a few units of few rows take, and some 40
+    // of many rows, whose parts are larger (us, shared / whole: 32 x 8192 x 8192 21.8 / 27.1, 32 x 8192 x 28672 49.4 / 44.4 with 15 of 64 units to save, 96 x 18176 x
+    // 4544 38.7 / 56.4, 128 x 28672 x 8192 72.7 / 88.8, 256 x 28672 x 8192 108.6 / 93.0 with 30 of 224).
+    p.stream_min = R < BM ? 4 : 16;
+    p.stream_gain = m.x.ptr ? 8 : p.Kb / 3 > (R < BM ? 8 : 40) ? p.Kb / 3 : R < BM ? 8 : 40;
+    p.tickets = m.tickets;
+    p.partials = m.partials;
+    p.partial_rows = partial_rows(m.rows);
     p.ct = m.gated ? p.Nb : (p.Nb + W - 1) / W;
-    p.a_rows = (int)(f8_rows_padded(m.rows) < BM ? f8_rows_padded(m.rows) : BM);
+    p.tile_rows = m.x.ptr ? 8 : R;
+    p.a_rows = (int)(f8_rows_padded(m.rows) < p.tile_rows ? f8_rows_padded(m.rows) : p.tile_rows);
     p.stage_bytes = p.a_rows * kF8Block + W * kF8BlockBytes;
-    const int extra = (m.gated ? 2 * BM * 4 : 0) + (m.experts ? 4 * (2 * m.experts + 1) : 0) + 1024;
+    const int extra = (R < BM ? p.tile_rows * 128 * W * 4 : m.gated ? 2 * BM * 4 : 0) + (m.experts ? 4 * (2 * m.experts + 1) : 0) + 1024;
     p.stages = (kSmemLimit - extra) / p.stage_bytes;
     if (p.stages > kMaxStages) p.stages = kMaxStages;
-    p.act = m.act; p.out_dtype = m.out_dtype; p.out_row_major = m.out_row_major; p.bias_row_major = m.bias_row_major;
+    if (p.stages < (R < BM ? (W * R > 64 ? 2 : 4) : 4 / W)) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: no room for the ring");
+    p.out_dtype = m.out_dtype; p.out_row_major = m.out_row_major; p.bias_row_major = m.bias_row_major;
     // 16 neighbouring columns of a row start at a multiple of this many bytes
     p.out_aligned = 0;
     if (!m.gated && (reinterpret_cast<uintptr_t>(m.out) & 15) == 0 && (!m.out_row_major || m.N * (m.out_dtype == TTB_FLOAT32 ? 4 : 2) % 16 == 0)) p.out_aligned = 16;
     p.wait_limit = barrier_limit_kcycles();
     if (int32_t rc = status_word_address(&p.status)) return rc;
-    int dev = 0, sms = 0;
+    int dev = 0;
     TTB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: device index %d is out of range", dev);
-    TTB_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    const int64_t most = (f8_rows_padded(m.rows) / BM + 1 + m.experts) * (int64_t)p.ct;   // an upper bound for a grouped matmul
-    if (most > INT32_MAX / 2) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: too many output tiles");
-    const int grid = most < sms ? (int)most : sms, smem = p.stages * p.stage_bytes + extra;
-    return m.gated ? launch<2, true>(p, grid, smem, dev, stream) : launch<1, false>(p, grid, smem, dev, stream);
+    if (sms * 16 > kF8TicketBytes) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: too many multiprocessors");
+    const int64_t most = (f8_rows_padded(m.rows) / p.tile_rows + 1 + m.experts) * (int64_t)p.ct;   // an upper bound for a grouped matmul
+    if (most > INT32_MAX / 2 || (uint64_t)sms * sms * p.Kb > 0xffffffffu) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: too many output tiles");
+    const int grid = most * p.Kb / p.stream_min < sms ? (int)(most * p.Kb / p.stream_min > most ? most * p.Kb / p.stream_min : most) : sms, smem = p.stages * p.stage_bytes + extra;
+    if (R < BM) return launch_matmul_float8_few(p, m.act, W, R, m.gated, grid, smem, dev, stream);
+    TTB_DISPATCH_ACT(m.act, return m.gated ? (launch<ACT, 2, true>(p, grid, smem, dev, stream)) : W == 2 ? (launch<ACT, 2, false>(p, grid, smem, dev, stream)) : (launch<ACT, 1, false>(p, grid, smem, dev, stream)));
+    return TTB_OK;
 }
 
 }  // namespace ttb
@@ -449,6 +480,9 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
 using ttb::fail;
 
 namespace {
+// The head of the workspace is that of ttb_matmul: arrival counters, of which the float8 kernels use the first kF8TicketBytes, and its accumulation tiles, which
+// they leave alone.
+constexpr int64_t kWorkspaceHead = 65536 + (int64_t(16) << 20);
 constexpr int64_t kMaxExtent = int64_t(1) << 24;   // rows, K and N: tile coordinates and row indexes stay far inside 32 bits
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -472,8 +506,8 @@ extern "C" {
 
 int64_t ttb_linear_float8_workspace_bytes(int64_t rows, int64_t K, int64_t N) {
     if (rows <= 0 || K <= 0 || N <= 0 || rows > kMaxExtent || K > kMaxExtent || N > kMaxExtent) return -1;
-    int64_t at = 0;
-    place(nullptr, at, rows, K);
+    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows, false);
+    if (!ttb::f8_quantises_itself(rows, 0)) place(nullptr, at, rows, K);
     return at;
 }
 
@@ -481,7 +515,7 @@ int32_t ttb_linear_float8(const void *a, const void *w_codes, const void *w_scal
                           int64_t N, int32_t activation, int32_t flags, void *workspace, int64_t workspace_bytes, void *stream) {
     if (!a || !w_codes || !w_scales || !out) return fail(TTB_E_INVALID, "ttb_linear_float8: null tensor pointer");
     if (out_dtype != TTB_BFLOAT16 && out_dtype != TTB_FLOAT32) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: output must be bfloat16 or float32");
-    if (flags & ~(TTB_MM_A_ROW_MAJOR | TTB_MM_OUT_ROW_MAJOR | TTB_MM_BIAS_ROW_MAJOR)) return fail(TTB_E_INVALID, "ttb_linear_float8: unknown flags %d", flags);
+    if (flags & ~(TTB_MM_A_ROW_MAJOR | TTB_MM_OUT_ROW_MAJOR | TTB_MM_BIAS_ROW_MAJOR | TTB_MM_WORKSPACE_ZEROED | TTB_MM_WEIGHTS_RESIDENT)) return fail(TTB_E_INVALID, "ttb_linear_float8: unknown flags %d", flags);
     if (activation < TTB_ACT_NONE || activation > TTB_ACT_SILU) return fail(TTB_E_INVALID, "ttb_linear_float8: unknown activation %d", activation);
     const int64_t need = ttb_linear_float8_workspace_bytes(rows, K, N);
     if (need < 0) return fail(TTB_E_INVALID, "ttb_linear_float8: rows, K and N must be between 1 and 2^24");
@@ -492,7 +526,9 @@ int32_t ttb_linear_float8(const void *a, const void *w_codes, const void *w_scal
         return fail(TTB_E_INVALID, "ttb_linear_float8: activations and codes must be 16-byte aligned, the other tensors as their elements");
     if (!ttb::workspace_serves(workspace, workspace_bytes, need)) return fail(TTB_E_WORKSPACE, "ttb_linear_float8: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     ttb::F8Matmul m = {};
-    int64_t at = 0;
+    m.tickets = static_cast<int32_t *>(workspace);
+    m.partials = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kWorkspaceHead);
+    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows, false);
     m.a = place(static_cast<uint8_t *>(workspace), at, rows, K);
     m.w[0] = {w_codes, static_cast<const float *>(w_scales)};
     m.rows = rows; m.K = K; m.N = N;
@@ -500,7 +536,17 @@ int32_t ttb_linear_float8(const void *a, const void *w_codes, const void *w_scal
     m.out = out; m.out_dtype = out_dtype; m.out_row_major = out_rm;
     m.bias = static_cast<const uint16_t *>(bias);
     m.bias_row_major = flags & TTB_MM_BIAS_ROW_MAJOR;
-    if (int32_t rc = ttb::launch_quantize_operand(a, a_rm, 1, rows, K, m.a, nullptr, 1, nullptr, 0, (cudaStream_t)stream)) return rc;
+    if (!(flags & TTB_MM_WORKSPACE_ZEROED)) TTB_CUDA_TRY(cudaMemsetAsync(workspace, 0, ttb::kF8TicketBytes, (cudaStream_t)stream));
+    const bool early = flags & TTB_MM_WEIGHTS_RESIDENT;
+    if (ttb::f8_quantises_itself(rows, 0)) {
+        m.a = {};
+        m.x = {static_cast<const uint16_t *>(a), nullptr, a_rm ? K : (K + 31) / 32 * 1024, !a_rm};
+        m.early = early;
+    } else {
+        // (a quantiser that does not let the matmul start at once lets it when all that came before has ended)
+        if (int32_t rc = ttb::launch_quantize_operand(a, a_rm, 1, rows, K, m.a, nullptr, 1, early, (cudaStream_t)stream)) return rc;
+        m.early = true;
+    }
     return ttb::launch_matmul_float8(m, (cudaStream_t)stream);
 }
 

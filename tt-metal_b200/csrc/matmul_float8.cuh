@@ -12,6 +12,14 @@ struct F8Activation {
     int64_t scale_pitch;
 };
 
+// bfloat16 rows that a kernel quantises itself: row r is row_of[r] of `ptr` (null: r itself).
+struct F8Rows {
+    const uint16_t *ptr;
+    const int32_t *row_of;
+    int64_t row_pitch;   // row-major: elements of a row; tiled: elements of a row of tiles
+    bool tiled;
+};
+
 struct F8Weight {
     const void *codes;   // [experts, N, K], row-major
     const float *scales; // [experts, ceil(N / 128), ceil(K / 128)]
@@ -20,6 +28,8 @@ struct F8Weight {
 // act(x w^T + bias) of all rows with one weight, or of runs of rows with an expert's weight each.
 struct F8Matmul {
     F8Activation a;
+    F8Rows x;                // few rows: instead of `a`, where its ptr is not null
+    bool early;              // weights and offsets are complete before the kernel before lets this one start
     F8Weight w[2];           // the second: the up projection of a gated pair
     int64_t rows, K, N;
     int experts;             // 0: one weight for all rows
@@ -34,11 +44,19 @@ struct F8Matmul {
     // or act(x w0^T) * (x w1^T), quantised again
     bool gated;
     F8Activation h;
+    // scratch for tiles whose K range several blocks share
+    int32_t *tickets;   // kF8TicketBytes, zero when the kernel starts and when it ends
+    float *partials;    // f8_partial_bytes, no particular contents
 };
+constexpr int64_t kF8TicketBytes = 8192;
+int64_t f8_partial_bytes(int64_t rows, bool gated);
 int32_t launch_matmul_float8(const F8Matmul &p, cudaStream_t stream);
+// Whether the kernel for these row counts quantises the activations itself.
+bool f8_quantises_itself(int64_t rows, int64_t experts);
 
-// Quantises [outer, H, K] bfloat16 rows into `out`: row r to row r, or (pos) to the rows pos[r * k + j] >= 0. Also clears zero[0 .. zeros - 1].
+// Quantises [outer, H, K] bfloat16 rows into `out`: row r to row r, or (pos) to the rows pos[r * k + j] >= 0. `early`: lets the next kernel start at once, else
+// when all that came before this one has ended.
 int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, int64_t H, int64_t K, const F8Activation &out, const int32_t *pos, int k,
-                                int32_t *zero, int zeros, cudaStream_t stream);
+                                bool early, cudaStream_t stream);
 
 }  // namespace ttb

@@ -120,9 +120,10 @@ Tensor linear_float8(const Tensor &x, const Float8 &w, const std::optional<Tenso
     const int64_t rows = outer * (x.layout() == Layout::TILE ? (H + 31) / 32 * 32 : H);
     auto outb = allocate_device_buffer(dev, physical_bytes(out_shape, out_dtype, x.layout()));
     const int64_t need = ttb_linear_float8_workspace_bytes(rows, K, N);
-    auto ws = need > 0 ? allocate_device_buffer(dev, need) : nullptr;   // handed back on return: later work on it is later on the stream
-    check(ttb_linear_float8(x.data(), w.codes.data(), w.scales.data(), bias_ptr, outb->ptr, static_cast<int>(out_dtype), rows, K, N, act, flags, ws ? ws->ptr : nullptr,
-                            need, nullptr),
+    void *ws = need > 0 ? dev->workspace(need) : nullptr;
+    // A float8 weight is written by a copy or by the quantiser, which lets no later kernel start before it has ended: it is complete before any kernel that this one may overlap.
+    check(ttb_linear_float8(x.data(), w.codes.data(), w.scales.data(), bias_ptr, outb->ptr, static_cast<int>(out_dtype), rows, K, N, act,
+                            flags | TTB_MM_WORKSPACE_ZEROED | TTB_MM_WEIGHTS_RESIDENT, ws, need, nullptr),
           op);
     return Tensor(outb, out_shape, out_dtype, x.layout());
 }
