@@ -1,7 +1,8 @@
 // Mixture of experts: the router (scores, groups, top-k, weights) and the experts' gated MLP on float8 weights.
 //
-// Router. A warp takes a row. An expert's choice value is its logit where that orders the scores (no bias, no sum over a group), else score + bias in
-// 64 bits: two experts next to the border may differ by less than 32 bits show, and the choice is a whole number. Ties go to the lowest index.
+// Router. A warp takes a row. An expert's choice value is its logit where that orders the scores (no bias, no sum over a group), else score + bias, first in 32
+// bits and, for the rows where two values that decide lie closer than that tells, again in 64: the choice is a whole number and has to be that of exact
+// values. Ties go to the lowest index. Bound by instructions, not by the logits' bytes. (All rows in 64 bits: 22 us for 8191 rows of 128.)
 //
 // The MLP y[t] = sum_j p[t, j] * down_e( q(act(gate_e x) * (up_e x)) ), e = ids[t, j], runs as
 //   plan      every assignment (t, j) gets a row, sorted by expert and then by t * k + j, with no room between the experts (the matmul's row tiles start at
@@ -44,6 +45,90 @@ __device__ __forceinline__ void best_of_warp(double &v, int &i) {   // the large
         if (w > v || (w == v && j < i)) { v = w; i = j; }
     }
 }
+// The same for 32-bit values, as two integer reductions: a larger value has the larger ordered().
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);   // (one zero)
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ void best_of_warp(float &v, int &i) {
+    const uint32_t u = ordered(v), top = __reduce_max_sync(0xffffffffu, u);
+    i = __reduce_min_sync(0xffffffffu, u == top ? i : kMaxExperts);
+    v = from_ordered(top);
+}
+
+// The chosen experts of one row, one a lane: lane j keeps the j-th (index E: none). `x`: this lane's logits, `key`: choice values (-inf: not to be chosen).
+// MARGIN: also says whether no two values that decide something lie within `eps` of each other.
+template <typename K, int V, bool MARGIN>
+__device__ __forceinline__ bool choose(const RouteArgs &p, const float (&x)[V], K (&key)[V], K eps, K *mine, int lane, int &my_id, float &my_x, float &first) {
+    const K none = -CUDART_INF_F;
+    bool sure = true;
+    if (p.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i * 32 + lane < p.E) mine[i * 32 + lane] = key[i];
+        __syncwarp();
+        const int size = p.E / p.groups;
+        K v = none;
+        if (lane < p.groups) {
+            K second = none;
+            for (int i = 0; i < size; ++i) {
+                const K c = mine[lane * size + i];
+                if (c > v) { second = v; v = c; }
+                else if (c > second) second = c;
+            }
+            if (p.sum_of_two && second > none) v += second;
+        }
+        uint32_t kept = 0;
+        K last = none;
+        for (int g = 0; g <= p.top_groups && g < p.groups; ++g) {   // (one more than is kept, for the margin)
+            const bool free = lane < p.groups && !(kept >> lane & 1);
+            K b = free ? v : none;
+            int i = free ? lane : 64;
+            best_of_warp(b, i);
+            if (g == p.top_groups) {
+                if (MARGIN) sure = sure && (b == none || last - b > 2 * eps);
+                break;
+            }
+            if (i < 32) kept |= 1u << i;
+            last = b;
+            if (!MARGIN && g + 1 == p.top_groups) break;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = i * 32 + lane;
+            if (e < p.E && !(kept >> (e / size) & 1)) key[i] = none;
+        }
+        __syncwarp();   // (`mine` may be written again)
+    }
+    my_id = p.E;
+    my_x = first = 0.0f;
+    K last = none;
+    for (int j = 0; j <= p.k; ++j) {
+        if (!MARGIN && j == p.k) break;
+        K b = none;
+        int id = kMaxExperts;
+        float bx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (key[i] > b) { b = key[i]; id = i * 32 + lane; bx = x[i]; }
+        const int own = id;
+        best_of_warp(b, id);
+        if (b == none) break;   // nothing is left
+        if (MARGIN && j > 0) sure = sure && last - b > eps;
+        last = b;
+        if (j == p.k) break;
+        bx = __shfl_sync(0xffffffffu, bx, id & 31);
+        if (own == id) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i * 32 + lane == id) key[i] = none;
+        }
+        if (lane == j) { my_id = id; my_x = bx; }
+        first = j == 0 ? bx : fmaxf(first, bx);
+    }
+    return sure;
+}
 
 // V: logits per lane.
 template <int V>
@@ -53,7 +138,6 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
     const int64_t r = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (r >= p.rows) return;
     const int64_t o = r / p.H, h = r - o * p.H;
-    const double none = -CUDART_INF;
     float x[V];
     bool nan = false;
     float most = -CUDART_INF_F;
@@ -69,86 +153,64 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
         }
     }
     nan = __any_sync(0xffffffffu, nan);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    // the softmax's denominator, where scores are needed (not for the shares among the chosen ones)
+    most = from_ordered(__reduce_max_sync(0xffffffffu, ordered(most)));
     const bool by_score = p.bias != nullptr || (p.groups > 1 && p.sum_of_two);
+    double *const mine = choice_smem + (size_t)warp * p.E;
+    auto is_free = [&](int i) { return i * 32 + lane < p.E && x[i] > -CUDART_INF_F; };   // (false for a NaN)
+    int my_id;
+    float my_x, first, key[V];
+    bool sure;
+    if (!by_score) {   // the logits order the scores
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = is_free(i) ? x[i] : -CUDART_INF_F;
+        sure = choose<float, V, false>(p, x, key, 0.0f, reinterpret_cast<float *>(mine), lane, my_id, my_x, first);
+    } else {
+        // In 32 bits first. A score is off by at most 2^-20 of 1 (exp, a sum of up to 1024 terms, a division), the sum with the bias by 2^-24 of itself.
+        float total = 1.0f, size = 1.0f;
+        if (!p.sigmoid) {
+            total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (is_free(i)) total += expf(x[i] - most);
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            key[i] = -CUDART_INF_F;
+            if (is_free(i)) {
+                const float s = p.sigmoid ? 1.0f / (1.0f + expf(-x[i])) : expf(x[i] - most) / total, b = p.bias ? p.bias[i * 32 + lane] : 0.0f;
+                key[i] = s + b == s + b ? s + b : -CUDART_INF_F;
+                if (fabsf(b) < CUDART_INF_F) size = fmaxf(size, fabsf(b));
+            }
+        }
+        size = from_ordered(__reduce_max_sync(0xffffffffu, ordered(size)));
+        sure = choose<float, V, true>(p, x, key, size * 0x1p-18f, reinterpret_cast<float *>(mine), lane, my_id, my_x, first);
+    }
     double total = 1.0;
-    if (!p.sigmoid && (by_score || !p.renormalize)) {
+    if (!p.sigmoid && (!sure || !p.renormalize)) {
         total = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i * 32 + lane < p.E && x[i] > -CUDART_INF_F) total += exp((double)x[i] - (double)most);
+            if (is_free(i)) total += exp((double)x[i] - (double)most);
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     }
     auto score = [&](float v) { return p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)most) / total; };
-    double key[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int e = i * 32 + lane;
-        key[i] = none;
-        if (e < p.E && x[i] > -CUDART_INF_F) {   // (false for a NaN)
-            key[i] = by_score ? score(x[i]) + (p.bias ? (double)p.bias[e] : 0.0) : (double)x[i];
-            if (key[i] != key[i]) key[i] = none;
-        }
-    }
-    if (p.groups > 1) {
-        double *mine = choice_smem + (size_t)warp * p.E;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i * 32 + lane < p.E) mine[i * 32 + lane] = key[i];
-        __syncwarp();
-        const int size = p.E / p.groups;
-        double v = none;
-        if (lane < p.groups) {
-            double second = none;
-            for (int i = 0; i < size; ++i) {
-                const double c = mine[lane * size + i];
-                if (c > v) { second = v; v = c; }
-                else if (c > second) second = c;
-            }
-            if (p.sum_of_two && second > none) v += second;
-        }
-        uint32_t kept = 0;
-        for (int g = 0; g < p.top_groups; ++g) {
-            double b = v;
-            int i = (lane < p.groups && !(kept >> lane & 1)) ? lane : 64;
-            if (i == 64) b = none;
-            best_of_warp(b, i);
-            if (i < 32) kept |= 1u << i;
-        }
+    if (!sure) {   // two values next to each other: again in 64 bits
+        double key64[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int e = i * 32 + lane;
-            if (e < p.E && !(kept >> (e / size) & 1)) key[i] = none;
+            key64[i] = -CUDART_INF;
+            if (is_free(i)) {
+                const double s = score(x[i]) + (p.bias ? (double)p.bias[i * 32 + lane] : 0.0);
+                if (s == s) key64[i] = s;
+            }
         }
+        choose<double, V, false>(p, x, key64, 0.0, mine, lane, my_id, my_x, first);
     }
-    // the k best, one after the other; lane j keeps the j-th
-    int my_id = p.E;
-    float my_x = 0.0f;
-    double first = 0.0;   // the largest logit among the chosen
-    for (int j = 0; j < p.k; ++j) {
-        double b = none;
-        int id = kMaxExperts;
-        float bx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (key[i] > b) { b = key[i]; id = i * 32 + lane; bx = x[i]; }
-        const int own = id;
-        best_of_warp(b, id);
-        if (id == kMaxExperts) break;   // nothing is left
-        bx = __shfl_sync(0xffffffffu, bx, id & 31);
-        if (own == id) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i * 32 + lane == id) key[i] = none;
-        }
-        if (lane == j) { my_id = id; my_x = bx; }
-        first = j == 0 ? (double)bx : fmax(first, (double)bx);
-    }
-    double w = 0.0;
-    if (my_id < p.E) w = !p.sigmoid && p.renormalize && !by_score ? exp((double)my_x - first) : score(my_x);
+    double w = 0.0;   // (the softmax's denominator drops out of shares)
+    if (my_id < p.E) w = p.renormalize && !p.sigmoid ? exp((double)my_x - (by_score ? (double)most : (double)first)) : score(my_x);
     if (p.renormalize) {
         double sum = w;
 #pragma unroll
@@ -220,12 +282,23 @@ __global__ void __launch_bounds__(256) combine_kernel(const float *y, const int3
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (h < H && c < hidden) {
             const int64_t r = o * H + h;
-            for (int j = 0; j < k; ++j) {
-                const int32_t at = __ldcg(pos + r * k + j);
-                if (at < 0) continue;
-                const float w = weights[r * k + j];
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(y + (int64_t)at * hidden + c));
-                s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+            for (int j0 = 0; j0 < k; j0 += 4) {   // four of the token's rows under way together
+                int32_t at[4];
+                float w[4];
+                float4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    at[j] = j0 + j < k ? __ldcg(pos + r * k + j0 + j) : -1;
+                    w[j] = j0 + j < k ? weights[r * k + j0 + j] : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at[j] >= 0) v[j] = __ldcg(reinterpret_cast<const float4 *>(y + (int64_t)at[j] * hidden + c));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at[j] >= 0) {
+                        s.x = fmaf(w[j], v[j].x, s.x); s.y = fmaf(w[j], v[j].y, s.y); s.z = fmaf(w[j], v[j].z, s.z); s.w = fmaf(w[j], v[j].w, s.w);
+                    }
             }
         }
         uint16_t *dst = out + (row_major ? pr * width + c : o * Hp * width + tiled_offset(h, c, width >> 5));
