@@ -224,49 +224,70 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
 }
 
 // Block e: the rows of expert e. ids outside [0, E) get no row. row_of: the row of the activations (of a tiled tensor: with its padding) that a row is from.
-__global__ void __launch_bounds__(256) plan_kernel(const int32_t *ids, int64_t assignments, int E, int k, int H, int Hp, int32_t *offsets, int32_t *pos, int32_t *row_of, int32_t *zero,
-                                                   int zeros) {
+// Every block looks through all ids, eight neighbours a thread (so that the loads of 8192 are under way together): first for those of the experts before e, whose
+// rows come first, then for its own. (One id a thread and step took 51 us for 16384 assignments.)
+constexpr int kPlanThreads = 1024, kPlanIds = 8;
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *ids, int64_t assignments, int E, int k, int H, int Hp, int32_t *offsets, int32_t *pos, int32_t *row_of,
+                                                            int32_t *zero, int zeros) {
     grid_dep_wait();
     grid_dep_launch();
-    __shared__ int warp_sum[8];
-    __shared__ int base_word;
+    __shared__ int warp_sum[2][32];
     const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int i = e * 256 + threadIdx.x; i < zeros; i += gridDim.x * 256) zero[i] = 0;
-    // rows of the experts before this one
-    int below = 0;
-    for (int64_t i = threadIdx.x; i < assignments; i += 256) {
-        const int x = ids[i];
-        below += x >= 0 && x < e;
-        if (e == 0 && (x < 0 || x >= E)) pos[i] = -1;
+    for (int i = e * kPlanThreads + threadIdx.x; i < zeros; i += gridDim.x * kPlanThreads) zero[i] = 0;
+    const bool vector = (reinterpret_cast<uintptr_t>(ids) & 15) == 0;
+    auto load = [&](int64_t i, int (&x)[kPlanIds]) {   // behind the end: -1
+        if (vector && i + kPlanIds <= assignments) {
+#pragma unroll
+            for (int q = 0; q < kPlanIds; q += 4) {
+                const int4 v = __ldcg(reinterpret_cast<const int4 *>(ids + i + q));
+                x[q] = v.x; x[q + 1] = v.y; x[q + 2] = v.z; x[q + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < kPlanIds; ++q) x[q] = i + q < assignments ? __ldcg(ids + i + q) : -1;
+        }
+    };
+    constexpr int64_t step = kPlanThreads * kPlanIds;
+    int below = 0, x[kPlanIds];
+    for (int64_t i = (int64_t)threadIdx.x * kPlanIds; i < assignments; i += step) {
+        load(i, x);
+#pragma unroll
+        for (int q = 0; q < kPlanIds; ++q) {
+            below += x[q] >= 0 && x[q] < e;
+            if (e == 0 && i + q < assignments && (x[q] < 0 || x[q] >= E)) pos[i + q] = -1;
+        }
     }
     below = __reduce_add_sync(0xffffffffu, below);
-    if (lane == 0) warp_sum[warp] = below;
+    if (lane == 0) warp_sum[0][warp] = below;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int w = 0; w < 8; ++w) s += warp_sum[w];
-        base_word = s;
-        offsets[e] = s;
-    }
-    __syncthreads();
-    int next = base_word;
-    for (int64_t i0 = 0; i0 < assignments; i0 += 256) {
-        const int64_t i = i0 + threadIdx.x;
-        const bool mine = i < assignments && ids[i] == e;
-        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) warp_sum[warp] = __popc(votes);
-        __syncthreads();
-        int before = next;
-        for (int w = 0; w < 8; ++w) {
-            if (w < warp) before += warp_sum[w];
-            next += warp_sum[w];
+    int next = __reduce_add_sync(0xffffffffu, warp_sum[0][lane]);
+    if (threadIdx.x == 0) offsets[e] = next;
+    int buf = 1;
+    for (int64_t i0 = 0; i0 < assignments; i0 += step, buf ^= 1) {
+        const int64_t i = i0 + (int64_t)threadIdx.x * kPlanIds;
+        if (assignments > step || i0 > 0) load(i, x);   // (else they are there still)
+        else if (i >= assignments) load(i, x);
+        int mine = 0;
+#pragma unroll
+        for (int q = 0; q < kPlanIds; ++q) mine += x[q] == e;
+        int before = mine;   // rows of e up to and with this thread's
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += y;
         }
-        if (mine) {
-            const int at = before + __popc(votes & ((1u << lane) - 1)), row = (int)(i / k);
-            pos[i] = at;
-            row_of[at] = row / H * Hp + row % H;
-        }
-        __syncthreads();
+        if (lane == 31) warp_sum[buf][warp] = before;
+        __syncthreads();   // (the other buffer is free again: whoever reads it has come here)
+        const int s = warp_sum[buf][lane];
+        int at = next + before - mine + __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
+        next += __reduce_add_sync(0xffffffffu, s);
+#pragma unroll
+        for (int q = 0; q < kPlanIds; ++q)
+            if (x[q] == e && i + q < assignments) {
+                const int row = (int)((i + q) / k);
+                pos[i + q] = at;
+                row_of[at++] = row / H * Hp + row % H;
+            }
     }
     if (e == E - 1 && threadIdx.x == 0) offsets[E] = next;
 }
@@ -444,7 +465,7 @@ int32_t ttb_experts_mlp_float8(const void *x, const void *ids, const void *weigh
     const cudaStream_t s = (cudaStream_t)stream;
     const bool x_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;
     const ttb::Scratch w = ttb::lay_out(static_cast<uint8_t *>(workspace), rows, experts, k, hidden, ffn);
-    if (int32_t rc = ttb::launch_dependent(ttb::plan_kernel, (unsigned)experts, 256, s, "plan", (const int32_t *)ids, w.assignments, (int)experts, (int)k, (int)H,
+    if (int32_t rc = ttb::launch_dependent(ttb::plan_kernel, (unsigned)experts, ttb::kPlanThreads, s, "plan", (const int32_t *)ids, w.assignments, (int)experts, (int)k, (int)H,
                                            (int)(x_rm ? H : ttb::round_up32(H)), w.offsets, w.pos, w.row_of, w.gated_tickets, (int)(2 * ttb::kF8TicketBytes / 4)))
         return rc;
     ttb::F8Matmul m = {};

@@ -62,6 +62,48 @@ __device__ __forceinline__ void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, ui
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return (uint32_t)f32_to_bf16_bits(lo) | ((uint32_t)f32_to_bf16_bits(hi) << 16); }
 
+// a += r * f of two neighbours in one instruction (f holds the factor twice).
+__device__ __forceinline__ void fma_pair(float &a0, float &a1, uint32_t r0, uint32_t r1, uint64_t f) {
+    asm("{\n\t"
+        ".reg .b64 a, r;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 r, {%2, %3};\n\t"
+        "fma.rn.f32x2 a, r, %4, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t"
+        "}"
+        : "+f"(a0), "+f"(a1)
+        : "r"(r0), "r"(r1), "l"(f));
+}
+__device__ __forceinline__ uint64_t twice(float f) { return ((uint64_t)__float_as_uint(f) << 32) | __float_as_uint(f); }
+
+// Adds an accumulator's NC columns, times f0 (gated: the second half times f1), to the sums, 32 at a time, the next 32 on their way meanwhile. column(j): that of
+// sum j; free() is called as soon as the accumulator may be written again.
+template <int NC, bool GATED, typename C, typename F>
+__device__ __forceinline__ void add_accumulator(uint32_t t0, float f0, float f1, float (&acc)[NC], C column, F free) {
+    uint32_t r[2][32];
+    auto load = [&](int q, uint32_t (&v)[32]) {
+        uint32_t lo[16], hi[16];
+        tmem_ld16(t0 + column(q), lo);
+        tmem_ld16(t0 + column(q + 16), hi);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            v[j] = lo[j];
+            v[16 + j] = hi[j];
+        }
+    };
+    load(0, r[0]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int q = 0; q < NC; q += 32) {
+        if (q + 32 < NC) load(q + 32, r[(q / 32 + 1) & 1]);
+        else free();
+        const uint64_t f = twice(GATED && q >= NC / 2 ? f1 : f0);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) fma_pair(acc[q + j], acc[q + j + 1], r[(q / 32) & 1][j], r[(q / 32) & 1][j + 1], f);
+        if (q + 32 < NC) tmem_ld_wait();
+    }
+}
+
 // A tile of the launch: rows [lo, hi) of expert e, kept as rows base .. base + tile_rows - 1 (base: at most lo), column tile c.
 struct Tile {
     int e, lo, hi, base, c;
@@ -129,9 +171,10 @@ struct Walk {
     int tile, whole, grid, u, u_end, Kb;
     int sharers, units;   // blocks that the shared tiles are dealt out to, their units
 
-    __device__ Walk(const Args &p, int tiles) {
+    __device__ Walk(const Args &p, int tiles) : Walk(p, tiles, (int)gridDim.x, (int)blockIdx.x) {}
+    __device__ Walk(const Args &p, int tiles, int blocks, int block) {
         Kb = p.Kb;
-        grid = (int)gridDim.x;
+        grid = blocks;
         const int left = tiles % grid;
         whole = tiles - left;
         units = left * Kb;
@@ -141,9 +184,9 @@ struct Walk {
             whole = tiles;
             units = sharers = 0;
         }
-        tile = (int)blockIdx.x;
-        u = (int)blockIdx.x < sharers ? first_unit((int)blockIdx.x) : 0;
-        u_end = (int)blockIdx.x < sharers ? first_unit((int)blockIdx.x + 1) : 0;
+        tile = block;
+        u = block < sharers ? first_unit(block) : 0;
+        u_end = block < sharers ? first_unit(block + 1) : 0;
     }
     // (the launcher keeps the products below 2^32; 64-bit divisions took a microsecond a piece where a hand-over waits for them)
     __device__ int first_unit(int block) const { return (int)((uint32_t)block * (uint32_t)units / (uint32_t)sharers); }
@@ -267,6 +310,114 @@ struct Meeting {
     }
 };
 
+constexpr int BM = 128;   // rows of a block's part of a tile in the many-rows kernels
+
+// 32 bytes, a whole sector.
+__device__ __forceinline__ void store8(void *dst, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// 16 columns from n on of one row.
+__device__ __forceinline__ void store16(const Args &p, int64_t row, int64_t n, const float *v) {
+    const int64_t width = p.out_row_major ? p.N : ((p.N + 31) & ~(int64_t)31);
+    if (n >= width) return;
+    const int64_t off = p.out_row_major ? row * p.N + n : tiled_offset(row, n, width >> 5);
+    uint32_t h[16];
+    const bool whole = n + 16 <= width;
+    if (p.out_dtype == TTB_FLOAT32) {
+        float *o = reinterpret_cast<float *>(p.out) + off;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) h[j] = __float_as_uint(v[j]);
+        if (p.out_aligned >= 32 && whole) {
+            store8(o, h);
+            store8(o + 8, h + 8);
+        } else if (p.out_aligned >= 16 && whole) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) reinterpret_cast<uint4 *>(o)[q] = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (n + j < width) o[j] = v[j];
+        }
+    } else {
+        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + off;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        if (p.out_aligned >= 32 && whole) {
+            store8(o, h);
+        } else if (p.out_aligned >= 16 && whole) {
+            reinterpret_cast<uint4 *>(o)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint4 *>(o)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (n + j < width) o[j] = f32_to_bf16_bits(v[j]);
+        }
+    }
+}
+
+// 16 columns from n on: bias, activation, store.
+template <int ACT>
+__device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, float *v) {
+    if (p.bias && n < p.N) {
+        const uint16_t *b = p.bias + (p.bias_row_major ? n : tiled_offset(0, n, p.N >> 5));   // (16 columns of the first tile row are neighbours)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (n + j < p.N) v[j] += __uint_as_float((uint32_t)__ldg(b + j) << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = apply_activation_t<ACT>(v[j]);
+    store16(p, row, n, v);
+}
+
+// A thread's columns of a whole tile. With an activation 16 at a time in a loop that shifts the sums down: 128 inlined activations are up to 60 KB of code, which
+// runs cold once a tile (a 350 x 4544 x 4672 launch with gelu: 39 us against 21 without finishing its tiles).
+template <int ACT, int NC>
+__device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n0, float (&acc)[NC]) {
+    if constexpr (ACT == TTB_ACT_NONE) {
+#pragma unroll
+        for (int q = 0; q < NC; q += 16) finish16<ACT>(p, row, n0 + q, acc + q);
+    } else {
+#pragma unroll 1
+        for (int q = 0; q < NC; q += 16) {
+            finish16<ACT>(p, row, n0 + q, acc);
+#pragma unroll
+            for (int j = 0; j + 16 < NC; ++j) acc[j] = acc[j + 16];
+        }
+    }
+}
+
+// act(g) * u; silu with the fast division (2 units in the last place; 0 where the exponential leaves its range, as it should be).
+template <int ACT>
+__device__ __forceinline__ float gate(float g, float u) {
+    if (ACT == TTB_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g)) * u;
+    return apply_activation_t<ACT>(g) * u;
+}
+
+// act(g) * u of one row's 64 columns from part * 64 on, quantised with the scale of all 128: the two warps of the rows exchange their largest magnitudes
+// through `red`.
+template <int ACT>
+__device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid, int c, int part, int lane_row, float (&acc)[128], float (*red)[BM], Meeting &meet) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        acc[j] = gate<ACT>(acc[j], acc[64 + j]);
+        m = fmaxf(m, fabsf(acc[j]));
+    }
+    red[part][lane_row] = m;
+    if (!meet(p)) return false;
+    const float scale = f8_scale(fmaxf(m, red[part ^ 1][lane_row])), inverse = __frcp_rn(scale);
+    if (!meet(p)) return false;   // (the next tile writes `red` again)
+    if (!valid) return true;
+#pragma unroll
+    for (int q = 0; q < 64; q += 16)
+        *reinterpret_cast<uint4 *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, part * 64 + q)) =
+            make_uint4(f8_pack4_by(acc + q, inverse), f8_pack4_by(acc + q + 4, inverse), f8_pack4_by(acc + q + 8, inverse), f8_pack4_by(acc + q + 12, inverse));
+    if (part == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
+    return true;
+}
+
 // Four columns from n (a multiple of four) on of one row.
 template <int ACT>
 __device__ __forceinline__ void finish4(const Args &p, int64_t row, int64_t n, float4 s) {
@@ -300,13 +451,12 @@ __device__ __forceinline__ void finish4(const Args &p, int64_t row, int64_t n, f
 template <int ACT, int W, bool GATED>
 __device__ __forceinline__ void finish_row_warp(const Args &p, int row, int c, int lane, const float4 (&s)[W]) {
     if constexpr (GATED) {
-        float h[4] = {apply_activation_t<ACT>(s[0].x) * s[W - 1].x, apply_activation_t<ACT>(s[0].y) * s[W - 1].y, apply_activation_t<ACT>(s[0].z) * s[W - 1].z,
-                      apply_activation_t<ACT>(s[0].w) * s[W - 1].w};
+        const float h[4] = {gate<ACT>(s[0].x, s[W - 1].x), gate<ACT>(s[0].y, s[W - 1].y), gate<ACT>(s[0].z, s[W - 1].z), gate<ACT>(s[0].w, s[W - 1].w)};
         float m = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         const float scale = f8_scale(m);
-        *reinterpret_cast<uint32_t *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, lane * 4)) = f8_pack4(h, scale);
+        *reinterpret_cast<uint32_t *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, lane * 4)) = f8_pack4_by(h, __frcp_rn(scale));
         if (lane == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
     } else {
 #pragma unroll

@@ -28,100 +28,6 @@ namespace {
 using namespace f8;
 using namespace ptx;
 
-constexpr int BM = 128;
-
-// 16 columns from n on of one row.
-__device__ __forceinline__ void store16(const Args &p, int64_t row, int64_t n, const float *v) {
-    const int64_t width = p.out_row_major ? p.N : ((p.N + 31) & ~(int64_t)31);
-    if (n >= width) return;
-    const int64_t off = p.out_row_major ? row * p.N + n : tiled_offset(row, n, width >> 5);
-    if (p.out_dtype == TTB_FLOAT32) {
-        float *o = reinterpret_cast<float *>(p.out) + off;
-        if (p.out_aligned >= 16 && n + 16 <= width) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) reinterpret_cast<float4 *>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (n + j < width) o[j] = v[j];
-        }
-    } else {
-        uint16_t *o = reinterpret_cast<uint16_t *>(p.out) + off;
-        if (p.out_aligned >= 16 && n + 16 <= width) {
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = (uint32_t)f32_to_bf16_bits(v[2 * j]) | ((uint32_t)f32_to_bf16_bits(v[2 * j + 1]) << 16);
-            reinterpret_cast<uint4 *>(o)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            reinterpret_cast<uint4 *>(o)[1] = make_uint4(h[4], h[5], h[6], h[7]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (n + j < width) o[j] = f32_to_bf16_bits(v[j]);
-        }
-    }
-}
-
-// 16 columns from n on: bias, activation, store.
-template <int ACT>
-__device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, float *v) {
-    if (p.bias && n < p.N) {
-        const uint16_t *b = p.bias + (p.bias_row_major ? n : tiled_offset(0, n, p.N >> 5));   // (16 columns of the first tile row are neighbours)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (n + j < p.N) v[j] += __uint_as_float((uint32_t)__ldg(b + j) << 16);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = apply_activation_t<ACT>(v[j]);
-    store16(p, row, n, v);
-}
-
-// A thread's columns of a whole tile. With an activation 16 at a time in a loop that shifts the sums down: 128 inlined activations are up to 60 KB of code, which
-// runs cold once a tile (a 350 x 4544 x 4672 launch with gelu: 39 us against 21 without finishing its tiles).
-template <int ACT, int NC>
-__device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n0, float (&acc)[NC]) {
-    if constexpr (ACT == TTB_ACT_NONE) {
-#pragma unroll
-        for (int q = 0; q < NC; q += 16) finish16<ACT>(p, row, n0 + q, acc + q);
-    } else {
-#pragma unroll 1
-        for (int q = 0; q < NC; q += 16) {
-            finish16<ACT>(p, row, n0 + q, acc);
-#pragma unroll
-            for (int j = 0; j + 16 < NC; ++j) acc[j] = acc[j + 16];
-        }
-    }
-}
-
-// act(g) * u of one row's 64 columns from part * 64 on, quantised with the scale of all 128: the two warps of the rows exchange their largest magnitudes
-// through `red`.
-template <int ACT>
-__device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid, int c, int part, int lane_row, float (&acc)[128], float (*red)[BM], Meeting &meet) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 64; ++j) {
-        acc[j] = apply_activation_t<ACT>(acc[j]) * acc[64 + j];
-        m = fmaxf(m, fabsf(acc[j]));
-    }
-    red[part][lane_row] = m;
-    if (!meet(p)) return false;
-    const float scale = f8_scale(fmaxf(m, red[part ^ 1][lane_row]));
-    if (!meet(p)) return false;   // (the next tile writes `red` again)
-    if (!valid) return true;
-#pragma unroll
-    for (int q = 0; q < 64; q += 16) {
-        float v[8], u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = acc[q + j];
-            u[j] = acc[q + 8 + j];
-        }
-        const uint2 x = f8_pack8(v, scale), y = f8_pack8(u, scale);
-        *reinterpret_cast<uint4 *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, part * 64 + q)) = make_uint4(x.x, x.y, y.x, y.y);
-    }
-    if (part == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
-    return true;
-}
-
 // 32 bytes, one sector.
 __device__ __forceinline__ void load_partial8(const float *src, float (&v)[8]) {
     asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -218,68 +124,84 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
         int s = 0, n = 0;
         uint32_t ph = 0;
         bool ok = true;
-        while (ok && walk.next(seg)) {
-            const Tile T = tile_of(p, off, cum, seg.tile);
+        // scales of a segment's first blocks: of this thread's row four blocks at a time, of the weight (the same for all threads) lane l that of block 32 i + l; both
+        // one step ahead, and the next segment's before this one's rows are finished
+        struct Scales {
+            const float *sa, *sw0, *sw1;
+            float4 xa, xa_next;
+            float w0, w0_next, w1, w1_next;
+        };
+        auto load_a = [&](const float *sa, int kb) { return kb < p.a.scale_pitch ? __ldcg(reinterpret_cast<const float4 *>(sa + kb)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+        auto load_w = [&](const float *sw, int kb) { return kb + lane < p.Kb ? __ldg(sw + kb + lane) : 0.0f; };
+        auto scales_of = [&](const Segment &g, const Tile &T) {
+            Scales c;
+            c.sa = p.a.scales + (int64_t)max(min(T.base + lane_row, T.hi - 1), T.lo) * p.a.scale_pitch;
+            const int64_t wrow = (int64_t)T.e * p.Nb + (GATED ? T.c : min(T.c * W + (W == 2 ? part : 0), p.Nb - 1));
+            c.sw0 = p.sw[0] + wrow * p.Kb;
+            c.sw1 = GATED ? p.sw[1] + wrow * p.Kb : nullptr;
+            c.xa = load_a(c.sa, g.kb0 & ~3);
+            c.xa_next = load_a(c.sa, (g.kb0 & ~3) + 4);
+            c.w0 = load_w(c.sw0, g.kb0 & ~31);
+            c.w0_next = load_w(c.sw0, (g.kb0 & ~31) + 32);
+            c.w1 = GATED ? load_w(c.sw1, g.kb0 & ~31) : 0.0f;
+            c.w1_next = GATED ? load_w(c.sw1, (g.kb0 & ~31) + 32) : 0.0f;
+            return c;
+        };
+        bool more = walk.next(seg);
+        Tile next_tile = {};
+        Scales next_scales = {};
+        if (more) {
+            next_tile = tile_of(p, off, cum, seg.tile);
+            next_scales = scales_of(seg, next_tile);
+        }
+        while (ok && more) {
+            const Segment now = seg;
+            const Tile T = next_tile;
+            Scales c = next_scales;
             const int row = T.base + lane_row;
             const bool valid = row >= T.lo && row < T.hi;
             const bool warp_valid = T.base + quad * 32 < T.hi && T.base + quad * 32 + 32 > T.lo;
-            // scales: of this thread's row four blocks at a time, of the weight (the same for all threads) lane l that of block 32 i + l; both one step ahead
-            const float *const sa = p.a.scales + (int64_t)max(min(row, T.hi - 1), T.lo) * p.a.scale_pitch;
-            const int64_t wrow = GATED ? T.c : min(T.c * W + (W == 2 ? part : 0), p.Nb - 1);
-            const float *const sw0 = p.sw[0] + ((int64_t)T.e * p.Nb + wrow) * p.Kb;
-            const float *const sw1 = GATED ? p.sw[1] + ((int64_t)T.e * p.Nb + wrow) * p.Kb : nullptr;
-            auto load_a = [&](int kb) { return kb < p.a.scale_pitch ? __ldcg(reinterpret_cast<const float4 *>(sa + kb)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
-            auto load_w = [&](const float *sw, int kb) { return kb + lane < p.Kb ? __ldg(sw + kb + lane) : 0.0f; };
-            float4 xa = load_a(seg.kb0 & ~3), xa_next = load_a((seg.kb0 & ~3) + 4);
-            float w0 = load_w(sw0, seg.kb0 & ~31), w0_next = load_w(sw0, (seg.kb0 & ~31) + 32);
-            float w1 = GATED ? load_w(sw1, seg.kb0 & ~31) : 0.0f, w1_next = GATED ? load_w(sw1, (seg.kb0 & ~31) + 32) : 0.0f;
             float acc[NC];
 #pragma unroll
             for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
-            for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
+            for (int kb = now.kb0; kb < now.kb1; ++kb, ++n) {
                 const int buf = n % NB;
-                const float x = (kb & 2) ? ((kb & 1) ? xa.w : xa.z) : ((kb & 1) ? xa.y : xa.x);
-                const float f0 = x * __shfl_sync(0xffffffffu, w0, kb & 31), f1 = GATED ? x * __shfl_sync(0xffffffffu, w1, kb & 31) : f0;
+                const float x = (kb & 2) ? ((kb & 1) ? c.xa.w : c.xa.z) : ((kb & 1) ? c.xa.y : c.xa.x);
+                const float f0 = x * __shfl_sync(0xffffffffu, c.w0, kb & 31), f1 = GATED ? x * __shfl_sync(0xffffffffu, c.w1, kb & 31) : f0;
                 if ((kb & 3) == 3) {
-                    xa = xa_next;
-                    xa_next = load_a(kb + 5);
+                    c.xa = c.xa_next;
+                    c.xa_next = load_a(c.sa, kb + 5);
                     if ((kb & 31) == 31) {
-                        w0 = w0_next;
-                        w0_next = load_w(sw0, kb + 33);
+                        c.w0 = c.w0_next;
+                        c.w0_next = load_w(c.sw0, kb + 33);
                         if (GATED) {
-                            w1 = w1_next;
-                            w1_next = load_w(sw1, kb + 33);
+                            c.w1 = c.w1_next;
+                            c.w1_next = load_w(c.sw1, kb + 33);
                         }
                     }
                 }
                 if (!__all_sync(0xffffffffu, mbar_wait(ring.done(s), ph, abort_flag, p.status, 54, wait_clocks(p)))) { ok = false; break; }
                 tc_fence_after_sync();
-                if (warp_valid) {
-                    const uint32_t t0 = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * 128 * W);
-#pragma unroll
-                    for (int q = 0; q < NC; q += 64 / W) {
-                        uint32_t r[4 / W][16];
-#pragma unroll
-                        for (int i = 0; i < 4 / W; ++i) tmem_ld16(t0 + column(q + 16 * i), r[i]);
-                        tmem_ld_wait();
-                        const float f = GATED && q >= 64 ? f1 : f0;
-#pragma unroll
-                        for (int i = 0; i < 4 / W; ++i)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) acc[q + 16 * i + j] = fmaf(__uint_as_float(r[i][j]), f, acc[q + 16 * i + j]);
-                    }
-                }
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ring.acc_empty(buf));
+                auto free = [&]() {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ring.acc_empty(buf));
+                };
+                if (warp_valid) add_accumulator<NC, GATED>(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * 128 * W), f0, f1, acc, column, free);
+                else free();
                 if (++s == p.stages) { s = 0; ph ^= 1; }
             }
             if (!ok) break;
-            if (seg.kb1 - seg.kb0 < p.Kb) {
+            more = walk.next(seg);
+            if (more) {
+                next_tile = tile_of(p, off, cum, seg.tile);
+                next_scales = scales_of(seg, next_tile);
+            }
+            if (now.kb1 - now.kb0 < p.Kb) {
                 // ---- a shared tile ----
-                const Sharing sh(walk, seg);
+                const Sharing sh(walk, now);
                 const int tile_floats = p.partial_rows * 128 * W, mine = lane_row * (128 * W);
-                const bool last_segment = walk.u >= walk.u_end;
+                const bool last_segment = !more;
                 bool all_here = false;
                 if ((int)blockIdx.x == sh.c0 && last_segment) {
                     // The first of the sharers, which comes to this tile at the end of its range: the others mostly have been here long ago.
@@ -440,7 +362,6 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     p.Kb = (int)f8_blocks(m.K); p.Nb = (int)f8_blocks(m.N);
     const int sms = stream_blocks();
     const int R = rows_per_tile(m.rows, m.experts), W = m.gated ? 2 : weight_blocks(m, R, sms);
-    p.Kb = (int)f8_blocks(m.K);
     // Where tiles are shared (units a block takes at least; units that sharing has to save): the hand-over costs what a few units of few rows take, and some 40
     // of many rows, whose parts are larger (us, shared / whole: 32 x 8192 x 8192 21.8 / 27.1, 32 x 8192 x 28672 49.4 / 44.4 with 15 of 64 units to save, 96 x 18176 x
     // 4544 38.7 / 56.4, 128 x 28672 x 8192 72.7 / 88.8, 256 x 28672 x 8192 108.6 / 93.0 with 30 of 224).
@@ -458,9 +379,10 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     if (p.stages > kMaxStages) p.stages = kMaxStages;
     if (p.stages < (R < BM ? (W * R > 64 ? 2 : 4) : 4 / W)) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: no room for the ring");
     p.out_dtype = m.out_dtype; p.out_row_major = m.out_row_major; p.bias_row_major = m.bias_row_major;
-    // 16 neighbouring columns of a row start at a multiple of this many bytes
+    // 16 neighbouring columns of a row start at a multiple of this many bytes (0: stores by element)
     p.out_aligned = 0;
-    if (!m.gated && (reinterpret_cast<uintptr_t>(m.out) & 15) == 0 && (!m.out_row_major || m.N * (m.out_dtype == TTB_FLOAT32 ? 4 : 2) % 16 == 0)) p.out_aligned = 16;
+    for (int bytes = 16; bytes <= 32 && !m.gated; bytes *= 2)
+        if (reinterpret_cast<uintptr_t>(m.out) % bytes == 0 && (!m.out_row_major || m.N * (m.out_dtype == TTB_FLOAT32 ? 4 : 2) % bytes == 0)) p.out_aligned = bytes;
     p.wait_limit = barrier_limit_kcycles();
     if (int32_t rc = status_word_address(&p.status)) return rc;
     int dev = 0;
