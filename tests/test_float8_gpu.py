@@ -102,6 +102,107 @@ def test_linear_row_major(dev, rows, k, n, dtype, bias, act):
     ref.assert_within(got, want, tol, (rows, k, n))
 
 
+# one and two weight blocks a tile, tiles that several blocks share and whole ones, rings that go round, in each of the kernels' row ranges
+KERNELS = [(1, 8192, 8192), (1, 640, 16384), (3, 18176, 1152), (8, 4544, 18176), (20, 2048, 28672), (32, 8192, 2048), (48, 28672, 512), (64, 1024, 28672), (60, 4096, 1000),
+           (128, 18176, 512), (300, 8192, 640), (1500, 1024, 4096), (1280, 8192, 4096), (700, 256, 9000)]
+
+
+@pytest.mark.parametrize("rows,k,n", KERNELS)
+@pytest.mark.parametrize("dtype,act", [("bfloat16", "silu"), ("float32", None)])
+def test_linear_in_every_kernel(dev, rows, k, n, dtype, act):
+    g = torch.Generator(device="cuda").manual_seed(rows + k + n)
+    codes = (torch.randn(n, k, generator=g, device="cuda") * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = (torch.rand(ref.blocks(n), ref.blocks(k), generator=g, device="cuda") + 0.5) * (2.0 / 100 / k ** 0.5)
+    x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    b = torch.randn(1, n, generator=g, device="cuda").bfloat16()
+    w = ttnn.Float8Tensor(put(codes.cpu(), dev), put(scales.cpu(), dev))
+    xt, bt = put(x.cpu(), dev), put(b.cpu(), dev)
+    want, tol = ref.linear(x, codes, scales, b, act, getattr(torch, dtype))
+    first = None
+    for _ in range(3):   # (what a launch leaves behind must not show in the next)
+        y = ttnn.to_torch(ttnn.linear_float8(xt, w, bias=bt, activation=act, dtype=getattr(ttnn, dtype)))
+        assert first is None or same_bits(first, y)
+        first = y
+    ref.assert_within(first, want, tol, (rows, k, n))
+
+
+def test_linear_many_calls_behind_each_other():
+    """Twelve launches of a graph that overlap, each with a weight of its own and more units a block than the ring has stages."""
+    c = ref.lib()
+    g = torch.Generator(device="cuda").manual_seed(30)
+    n = k = 8192
+    x = torch.randn(1, k, generator=g, device="cuda").bfloat16()
+    ws = [((torch.randn(n, k, generator=g, device="cuda") * 100).clamp(-448, 448).to(torch.float8_e4m3fn), torch.rand(64, 64, generator=g, device="cuda") * 1e-3) for _ in range(4)]
+    outs = [torch.empty(1, n, dtype=torch.float32, device="cuda") for _ in range(12)]
+    need = c.ttb_linear_float8_workspace_bytes(1, k, n)
+    space = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+
+    def call(i):
+        w = ws[i % 4]
+        assert c.ttb_linear_float8(x.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), None, outs[i].data_ptr(), 1, 1, k, n, 0, 3 | cabi.MM_WORKSPACE_ZEROED | cabi.MM_WEIGHTS_RESIDENT,
+                                   space.data_ptr(), need, s.cuda_stream) == 0
+    call(0)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        for i in range(12):
+            call(i)
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        want, tol = ref.linear(x, *ws[i % 4], None, None, torch.float32)
+        ref.assert_within(out, want, tol, i)
+    assert int(space[:65536].count_nonzero()) == 0
+
+
+def test_linear_between_block_float_linears(dev):
+    """Both kinds share the device's scratch, whose counters each leaves at zero."""
+    g = gen(31)
+    x = ref.rows_of(g, 32, 2048)
+    w8 = ref.weight(g, 1024, 2048)
+    wb = torch.randn(2048, 4096, generator=g) * 0.02
+    xt, f8, bf = put(x, dev, ttnn.TILE_LAYOUT), pair(w8, dev), put(wb, dev, ttnn.TILE_LAYOUT, ttnn.bfloat8_b)
+    want, tol = ref.linear(x.cuda(), w8[0].cuda(), w8[1].cuda(), None, None, torch.bfloat16)
+    exact = x.double() @ ttnn.to_torch(bf).double()
+    near = (x.double().abs() @ wb.double().abs()) * 2.0 ** -7 + 1e-6
+    for _ in range(4):
+        a, b = ttnn.linear(xt, bf), ttnn.linear_float8(xt, f8)
+        assert ((ttnn.to_torch(a).double() - exact).abs() <= near).all()
+        ref.assert_within(ttnn.to_torch(b), want, tol)
+
+
+def test_linear_with_offsets_behind_32_bits(dev):
+    """A weight of more than 2^32 codes, and a result of more than 2^31 values."""
+    c = ref.lib()
+    g = torch.Generator(device="cuda").manual_seed(32)
+    n, k = 140000, 32768
+    codes = torch.empty(n, k, dtype=torch.float8_e4m3fn, device="cuda")
+    for part in codes.split(8192):
+        part.copy_((torch.randn(part.shape, generator=g, device="cuda") * 100).clamp_(-448, 448))
+    scales = (torch.rand(ref.blocks(n), ref.blocks(k), generator=g, device="cuda") + 0.5) * (2.0 / 100 / k ** 0.5)
+    pick = torch.tensor([0, 5, 65535, 131071, 131072, 131100, n - 1], device="cuda")
+    for rows in (1, 40):
+        x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+        out = torch.empty(rows, n, dtype=torch.float32, device="cuda")
+        ws = _workspace(c.ttb_linear_float8_workspace_bytes(rows, k, n))
+        _abi_linear(c, x, codes, scales, out, n, ws, dtype=1)
+        w = codes[pick].double() * scales.double()[pick // 128].repeat_interleave(128, 1)
+        want, tol = ref.sums(ref.requantized(x), w)
+        ref.assert_within(out[:, pick], want, tol + want.abs() * 2.0 ** -23, rows)
+    del codes, scales, out
+    rows, k, n = 70000, 128, 32768
+    x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    w = [t.cuda() for t in ref.weight(gen(33), n, k)]
+    out = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    _abi_linear(c, x, *w, out, n, _workspace(c.ttb_linear_float8_workspace_bytes(rows, k, n)))
+    for r in (0, 32767, 65535, 65536, 69999):
+        want, tol = ref.linear(x[r:r + 1], *w, None, None, torch.bfloat16)
+        ref.assert_within(out[r:r + 1], want, tol, r)
+
+
 @pytest.mark.parametrize("shape,n,act,dtype", [((1, 1, 5, 256), 160, None, "bfloat16"), ((2, 3, 33, 80), 70, "silu", "float32"), ((40, 4544), 4672, "relu", "bfloat16"),
                                                ((3, 32, 128), 128, "gelu", "float32"), ((1, 1, 150, 1040), 513, "silu", "bfloat16")])
 def test_linear_tiled(dev, shape, n, act, dtype):
@@ -321,7 +422,8 @@ def _expert_case(g, rows, e, k, hidden, ffn):
 
 
 EXPERTS = [(1, 1, 1, 16, 16), (1, 8, 2, 256, 128), (1, 64, 8, 2048, 1024), (3, 4, 2, 128, 144), (7, 5, 3, 272, 400), (33, 8, 2, 512, 272), (64, 3, 2, 256, 1200),
-           (100, 16, 4, 1040, 256), (130, 2, 1, 144, 384), (257, 4, 2, 640, 512), (300, 100, 8, 128, 128), (1000, 3, 2, 256, 256), (40, 1024, 3, 32, 48)]
+           (100, 16, 4, 1040, 256), (130, 2, 1, 144, 384), (257, 4, 2, 640, 512), (300, 100, 8, 128, 128), (1000, 3, 2, 256, 256), (40, 1024, 3, 32, 48),
+           (200, 1, 1, 8192, 384), (32, 2, 1, 4096, 512), (90, 2, 1, 512, 8192), (2000, 16, 8, 256, 384)]
 
 
 @pytest.mark.parametrize("rows,e,k,hidden,ffn", EXPERTS)
