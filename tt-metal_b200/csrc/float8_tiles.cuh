@@ -261,8 +261,9 @@ __device__ __forceinline__ void fetch(const Args &p, const Ring &ring, Walk walk
 }
 
 // Issuing warp `which` of kIssuers: every kIssuers-th unit. The ring has to have NB stages or more: the wait for a free accumulator says that the unit NB before
-// is over, and with it the stage's last use, whoever issued that; without it the parity of the wait for the stage would mean nothing. issue(stage address, accumulator, tile) issues the unit's MMAs.
-template <int NB, typename F>
+// is over, and with it the stage's last use, whoever issued that; without it the parity of the wait for the stage would mean nothing. FULL_FIRST: the ring has an even
+// number of stages, so that a stage is always the same warp's, and the waits may come the other way round. issue(stage address, accumulator, tile) issues the unit's MMAs.
+template <int NB, bool FULL_FIRST, typename F>
 __device__ __forceinline__ void issue_mmas(const Args &p, const Ring &ring, Walk walk, const int *off, const int *cum, int which, F issue) {
     grid_dep_wait();   // (the bounded waits are not to count the time of the kernel before)
     const bool leader = elect_one();
@@ -274,8 +275,11 @@ __device__ __forceinline__ void issue_mmas(const Args &p, const Ring &ring, Walk
         for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
             if (n % kIssuers == which) {
                 const int buf = n % NB;
-                if (!__all_sync(0xffffffffu, mbar_wait(ring.acc_empty(buf), (uint32_t)(((n / NB) & 1) ^ 1), ring.abort_flag, p.status, 52, wait_clocks(p))) ||
-                    !__all_sync(0xffffffffu, mbar_wait(ring.full(s), ph, ring.abort_flag, p.status, 53, wait_clocks(p))))
+                const uint32_t acc_parity = (uint32_t)(((n / NB) & 1) ^ 1);
+                auto wait_full = [&]() { return (bool)__all_sync(0xffffffffu, mbar_wait(ring.full(s), ph, ring.abort_flag, p.status, 53, wait_clocks(p))); };
+                // (what mostly comes last is waited for last)
+                if ((FULL_FIRST && !wait_full()) || !__all_sync(0xffffffffu, mbar_wait(ring.acc_empty(buf), acc_parity, ring.abort_flag, p.status, 52, wait_clocks(p))) ||
+                    (!FULL_FIRST && !wait_full()))
                     return;
                 tc_fence_after_sync();
                 if (leader) {

@@ -104,7 +104,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
         if (warp == kFetchWarp) {
             fetch<W, GATED, false, false>(p, ring, walk, off, cum);
         } else if (warp < kIssueWarp + kIssuers) {
-            issue_mmas<NB>(p, ring, walk, off, cum, warp - kIssueWarp, [&](uint32_t src, int buf, const Tile &) {
+            issue_mmas<NB, true>(p, ring, walk, off, cum, warp - kIssueWarp, [&](uint32_t src, int buf, const Tile &) {
                 const uint64_t a = smem_desc_sw128(src), b = smem_desc_sw128(src + (uint32_t)(p.a_rows * kF8Block));
 #pragma unroll
                 for (int k = 0; k < 4; ++k)   // 32 bytes of K further: two 16-byte units in the descriptor's address
@@ -377,6 +377,7 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     const int extra = (R < BM ? p.tile_rows * 128 * W * 4 : m.gated ? 2 * BM * 4 : 0) + (m.experts ? 4 * (2 * m.experts + 1) : 0) + 1024;
     p.stages = (kSmemLimit - extra) / p.stage_bytes;
     if (p.stages > kMaxStages) p.stages = kMaxStages;
+    if (R >= BM) p.stages &= ~1;   // (matmul_float8.cu: FULL_FIRST)
     if (p.stages < (R < BM ? (W * R > 64 ? 2 : 4) : 4 / W)) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: no room for the ring");
     p.out_dtype = m.out_dtype; p.out_row_major = m.out_row_major; p.bias_row_major = m.bias_row_major;
     // 16 neighbouring columns of a row start at a multiple of this many bytes (0: stores by element)

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     if (warp == kProducerWarp) {
         fetch<W, GATED, true, QUANT>(p, ring, walk, off, cum);
     } else if (warp >= kMmaWarp && warp < kMmaWarp + kIssuers) {
-        issue_mmas<NB>(p, ring, walk, off, cum, warp - kMmaWarp, [&](uint32_t src, int buf, const Tile &T) {
+        issue_mmas<NB, false>(p, ring, walk, off, cum, warp - kMmaWarp, [&](uint32_t src, int buf, const Tile &T) {
             const uint64_t x = smem_desc_sw128(src), w = smem_desc_sw128(src + (uint32_t)(p.a_rows * kF8Block));
             const uint32_t idesc = instr_desc_e4m3(128, (T.hi - T.base + 15) & ~15);
 #pragma unroll
