@@ -104,7 +104,8 @@ def test_linear_row_major(dev, rows, k, n, dtype, bias, act):
 
 # one and two weight blocks a tile, tiles that several blocks share and whole ones, rings that go round, in each of the kernels' row ranges
 KERNELS = [(1, 8192, 8192), (1, 640, 16384), (3, 18176, 1152), (8, 4544, 18176), (20, 2048, 28672), (32, 8192, 2048), (48, 28672, 512), (64, 1024, 28672), (60, 4096, 1000),
-           (128, 18176, 512), (300, 8192, 640), (1500, 1024, 4096), (1280, 8192, 4096), (700, 256, 9000)]
+           (128, 18176, 512), (300, 8192, 640), (1500, 1024, 4096), (1280, 8192, 4096), (700, 256, 9000),
+           (64, 18272, 6376), (126, 18272, 6376), (97, 9008, 2400)]
 
 
 @pytest.mark.parametrize("rows,k,n", KERNELS)

@@ -56,11 +56,11 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
     constexpr int NC = 64 * W;      // columns of an adding thread
     constexpr int NB = 4 / W;       // accumulators: all of tensor memory
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 10];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 11];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_word;
     __shared__ int tiles_word;
-    __shared__ volatile int ticket;
+    __shared__ volatile int ticket, pending;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint8_t *after = smem + p.stages * p.stage_bytes;
@@ -69,7 +69,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
     int *cum = off + p.experts + 1;
     const uint32_t bar0 = smem_u32(bars);
     auto pair = [&](int quad) { return bar0 + 8u * (2 * kMaxStages + 4 + quad); };
-    const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + 8), handed_bar = all_bar + 8;
+    const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + 8), handed_bar = all_bar + 8, told_bar = handed_bar + 8;
     volatile int *abort_flag = &abort_word;
     const Ring ring = {sbase, bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,6 +83,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
         for (int q = 0; q < 4; ++q) mbar_init(pair(q), 2);
         mbar_init(all_bar, kAddWarps);
         mbar_init(handed_bar, kAddWarps);
+        mbar_init(told_bar, 1);
         abort_word = 0;
         fence_mbar_init();
     }
@@ -113,7 +114,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
                     mma_e4m3_ss(tmem_base + (uint32_t)(buf * 128 * W), a + 2 * k, b + 2 * k, instr_desc_e4m3(BM, 128 * W), k > 0);
             });
         } else {
-            hand_over<ACT, W, GATED>(p, handed_bar, abort_flag, walk, off, cum);
+            hand_over<ACT, W, GATED, false>(p, handed_bar, told_bar, &pending, abort_flag, walk, off, cum);
         }
     } else {
         if (W == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
@@ -149,6 +150,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
             c.w1_next = GATED ? load_w(c.sw1, (g.kb0 & ~31) + 32) : 0.0f;
             return c;
         };
+        Segment handed = {-1, 0, 0};   // the shared tile that the hand-over warp has
         bool more = walk.next(seg);
         Tile next_tile = {};
         Scales next_scales = {};
@@ -208,9 +210,9 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
                 if ((int)blockIdx.x == sh.c0 && last_segment) {
                     // The first of the sharers, which comes to this tile at the end of its range: the others mostly have been here long ago.
                     if (threadIdx.x == 0) ticket = read_tickets(p.tickets + sh.q);
-                    if (!meet_all(p)) break;
+                    if (!meet_all(p)) { ok = false; break; }
                     all_here = ticket == sh.c1 - sh.c0;
-                    if (!meet_all(p)) break;   // (`ticket` is written again)
+                    if (!meet_all(p)) { ok = false; break; }   // (`ticket` is written again)
                 }
                 if (all_here) {
                     if (threadIdx.x == 0) p.tickets[sh.q] = 0;
@@ -239,11 +241,12 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
                     if (!last_segment) {   // the hand-over warp sees to the rest while the next segment runs
                         __syncwarp();
                         if (lane == 0) mbar_arrive(handed_bar);
+                        handed = now;
                         continue;
                     }
-                    if (!meet_all(p)) break;
+                    if (!meet_all(p)) { ok = false; break; }
                     if (threadIdx.x == 0) ticket = take_ticket(p.tickets + sh.q);
-                    if (!meet_all(p)) break;
+                    if (!meet_all(p)) { ok = false; break; }
                     if (ticket != sh.c1 - sh.c0) continue;
                     if (threadIdx.x == 0) p.tickets[sh.q] = 0;
                     // the last one adds them: row after row, each by a whole warp
@@ -258,6 +261,13 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
             } else {
                 if (valid) finish_row<ACT, NC>(p, row, (int64_t)T.c * 128 * W + part * NC, acc);
             }
+        }
+        if (ok && !more && handed.tile >= 0 && __all_sync(0xffffffffu, mbar_wait(told_bar, 0, abort_flag, p.status, 61, wait_clocks(p))) && pending >= 0) {
+            const Sharing sh(walk, handed);
+            const Tile T = tile_of(p, off, cum, handed.tile);
+            if (threadIdx.x == 0) p.tickets[sh.q] = 0;
+            auto part_of = [&](int block) { return sh.part(p, block, p.partial_rows * 128 * W); };
+            add_parts<ACT, W, GATED, 4, 2, kAddWarps>(p, part_of, sh.c0, sh.c1, T.lo - T.base + warp, T.hi - T.base, T.base, T.c, lane);
         }
     }
 
@@ -366,7 +376,7 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     const int R = rows_per_tile(m.rows, m.experts), W = m.gated ? 2 : weight_blocks(m, R, sms);
     // Where tiles are shared (units a block takes at least; units that sharing has to save): the hand-over costs what a few units of few rows take, and some 40
     // of many rows, whose parts are larger (us, shared / whole: 32 x 8192 x 8192 21.8 / 27.1, 32 x 8192 x 28672 49.4 / 44.4 with 15 of 64 units to save, 96 x 18176 x
-    // 4544 38.7 / 56.4, 128 x 28672 x 8192 72.7 / 88.8, 256 x 28672 x 8192 108.6 / 93.0 with 30 of 224).
+    // 4544 35.6 / 53.5, 128 x 28672 x 8192 65.7 / 83.7, 128 x 8192 x 20000 58.6 / 43.7 with 30 of 64, 256 x 28672 x 8192 101 / 93 with 30 of 224).
     p.stream_min = R < BM ? 4 : 16;
     p.stream_gain = m.x.ptr ? 8 : p.Kb / 3 > (R < BM ? 8 : 40) ? p.Kb / 3 : R < BM ? 8 : 40;
     p.tickets = m.tickets;

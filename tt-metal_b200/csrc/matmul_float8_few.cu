@@ -106,15 +106,16 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     static_assert(!QUANT || R == 32, "tiles of kQuantRows rows");
     constexpr int NR = R * W / 2;             // rows of an epilogue thread: all of them of weight block `half`, or half of the rows of the one block
     constexpr int NX = NR > 32 ? 2 : 1;       // registers that hold a scale of each
+    constexpr bool ADD = R <= 32;
     constexpr int RU = QUANT ? 1 : R == 32 ? 2 : 4 / W, BU = QUANT ? 8 / W : R == 32 ? 4 / W : 4;   // rows and blocks whose parts a warp adds at a time
     constexpr int NB = few_accumulators(W, R), kTmemCols = NB * W * R;
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + NB + 2 + kScaleSlots];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + NB + 3 + kScaleSlots];
     __shared__ float scales[QUANT ? kScaleSlots * 32 : 1];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_word;
     __shared__ int tiles_word;
-    __shared__ volatile int ticket;
+    __shared__ volatile int ticket, pending;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *sums = reinterpret_cast<float *>(smem + p.stages * p.stage_bytes);   // [tile_rows][128 W]
     int *off = reinterpret_cast<int *>(sums + p.tile_rows * 128 * W);
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     const uint32_t bar0 = smem_u32(bars);
     volatile int *abort_flag = &abort_word;
     const Ring ring = {smem_u32(smem), bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag};
-    const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + NB), handed_bar = all_bar + 8, ready0 = handed_bar + 8;
+    const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + NB), handed_bar = all_bar + 8, told_bar = handed_bar + 8, ready0 = told_bar + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -133,6 +134,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
         for (int b = 0; b < NB; ++b) mbar_init(ring.acc_empty(b), kEpiWarps);
         mbar_init(all_bar, kEpiWarps);
         mbar_init(handed_bar, kEpiWarps);
+        mbar_init(told_bar, 1);
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(ready0 + 8u * i, 1);
         abort_word = 0;
         fence_mbar_init();
@@ -165,13 +167,13 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     } else if (QUANT && warp >= kQuantWarp0) {
         quantise(p, ring, smem, ready0, scales, walk, off, cum, warp - kQuantWarp0);
     } else if (warp >= kMmaWarp + kIssuers) {
-        hand_over<ACT, W, GATED>(p, handed_bar, abort_flag, walk, off, cum);
+        hand_over<ACT, W, GATED, ADD>(p, handed_bar, told_bar, &pending, abort_flag, walk, off, cum);
     } else {
         grid_dep_wait();
         const int quad = warp & 3, half = warp >> 2;
         const int first_row = W == 1 ? half * NR : 0, block = W == 1 ? 0 : half;   // of this thread's sums
         Meeting meet = {all_bar, 0, abort_flag};
-        Segment seg;
+        Segment seg, handed = {-1, 0, 0};   // the shared tile that the hand-over warp has
         int s = 0, n = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
             const bool shared_tile = seg.kb1 - seg.kb0 < p.Kb, last_segment = walk.u >= walk.u_end;
             const int r0 = T.lo - T.base + warp;
             if (!shared_tile) {
-                if (!meet(p)) break;
+                if (!meet(p)) { ok = false; break; }
 #pragma unroll 1
                 for (int r = r0; r < rows; r += kEpiWarps) {
                     float4 v[W];
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
                 // The first of the sharers comes to this tile at the end of its range: the others mostly have been here long ago.
                 const bool first = (int)blockIdx.x == sh.c0 && last_segment;
                 if (first && threadIdx.x == 0) ticket = read_tickets(p.tickets + sh.q);
-                if (!meet(p)) break;
+                if (!meet(p)) { ok = false; break; }
                 if (first && ticket == sh.c1 - sh.c0) {
                     if (threadIdx.x == 0) p.tickets[sh.q] = 0;
                     add_parts<ACT, W, GATED, RU, BU, kEpiWarps>(p, part_of, sh.c0, sh.c1, r0, rows, T.base, T.c, lane, sums);
@@ -277,10 +279,11 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
                     if (!last_segment) {   // the hand-over warp sees to the rest while the next segment runs
                         __syncwarp();
                         if (lane == 0) mbar_arrive(handed_bar);
+                        handed = seg;
                     } else {
-                        if (!meet(p)) break;
+                        if (!meet(p)) { ok = false; break; }
                         if (threadIdx.x == 0) ticket = take_ticket(p.tickets + sh.q);
-                        if (!meet(p)) break;
+                        if (!meet(p)) { ok = false; break; }
                         if (ticket == sh.c1 - sh.c0) {   // the last one adds them
                             if (threadIdx.x == 0) p.tickets[sh.q] = 0;
                             add_parts<ACT, W, GATED, RU, BU, kEpiWarps>(p, part_of, sh.c0, sh.c1, r0, rows, T.base, T.c, lane);
@@ -288,7 +291,14 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
                     }
                 }
             }
-            if (!meet(p)) break;   // (the next tile's sums take the place of these)
+            if (!meet(p)) { ok = false; break; }   // (the next tile's sums take the place of these)
+        }
+        if (!ADD && ok && handed.tile >= 0 && __all_sync(0xffffffffu, mbar_wait(told_bar, 0, abort_flag, p.status, 61, wait_clocks(p))) && pending >= 0) {
+            const Sharing sh(walk, handed);
+            const Tile T = tile_of(p, off, cum, handed.tile);
+            if (threadIdx.x == 0) p.tickets[sh.q] = 0;
+            auto part_of = [&](int b) { return sh.part(p, b, p.partial_rows * 128 * W); };
+            add_parts<ACT, W, GATED, RU, BU, kEpiWarps>(p, part_of, sh.c0, sh.c1, T.lo - T.base + warp, T.hi - T.base, T.base, T.c, lane);
         }
     }
 
