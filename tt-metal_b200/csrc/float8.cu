@@ -8,6 +8,8 @@
 #include "matmul_float8.cuh"
 #include "sm100_ptx.cuh"
 
+#include <cuda_bf16.h>
+
 namespace ttb {
 namespace {
 
@@ -18,38 +20,69 @@ struct Source {
     bool tiled, vector; // vector: eight neighbours of a row are 16-byte aligned
 };
 
-// Columns c .. c + 7 of a row; what lies behind W is zero.
+// Columns c .. c + 7 of a row as they lie in memory; what lies behind W is zero.
 template <typename T>
-__device__ __forceinline__ void load8(const Source &s, int64_t o, int64_t row, int64_t c, int64_t W, float (&v)[8]) {
-    const T *p = reinterpret_cast<const T *>(s.ptr) + o * s.slab + (s.tiled ? tiled_offset(row, c, s.pitch) : row * s.pitch + c);
-    if (s.vector && c + 8 <= W) {
-        if (sizeof(T) == 4) {
-            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p)), b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(p));
-            const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ const T *place_of(const Source &s, int64_t o, int64_t row, int64_t c) {
+    return reinterpret_cast<const T *>(s.ptr) + o * s.slab + (s.tiled ? tiled_offset(row, c, s.pitch) : row * s.pitch + c);
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const Source &s, int64_t o, int64_t row, int64_t c) {   // all there and aligned
+    const uint4 *p = reinterpret_cast<const uint4 *>(place_of<T>(s, o, row, c));
+    Raw8<T> v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[2 * j] = __uint_as_float(h[j] << 16);
-                v[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
-            }
-        }
-        return;
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+        const uint4 a = __ldcg(p + j);
+        v.w[4 * j] = a.x; v.w[4 * j + 1] = a.y; v.w[4 * j + 2] = a.z; v.w[4 * j + 3] = a.w;
     }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const Source &s, int64_t o, int64_t row, int64_t c, int64_t W) {
+    if (s.vector && c + 8 <= W) return load8<T>(s, o, row, c);
+    constexpr int N = 2 * sizeof(T);   // words
+    const T *p = place_of<T>(s, o, row, c);
+    Raw8<T> v;
+    constexpr int per = 8 / N;   // values of a word
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        v.w[j] = 0;
+#pragma unroll
+        for (int q = 0; q < per; ++q)
+            if (c + j * per + q < W) {
+                if (sizeof(T) == 4) v.w[j] = reinterpret_cast<const uint32_t *>(p)[j];
+                else v.w[j] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[2 * j + q] << (16 * q);
+            }
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T> &r, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float x = 0.0f;
-        if (c + j < W) {
-            if (sizeof(T) == 4) x = reinterpret_cast<const float *>(p)[j];
-            else x = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << 16);
-        }
-        v[j] = x;
+        if (sizeof(T) == 4) v[j] = __uint_as_float(r.w[j % (2 * sizeof(T))]);
+        else v[j] = __uint_as_float(j & 1 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
     }
 }
 
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = 0.0f;
+// The largest magnitude; a NaN counts nothing.
+template <typename T>
+__device__ __forceinline__ float amax8(const Raw8<T> &r) {
+    if (sizeof(T) == 2) {
+        __nv_bfloat162 m[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = r.w[j] & 0x7fff7fffu;
+            m[j] = *reinterpret_cast<const __nv_bfloat162 *>(&w);
+        }
+        const __nv_bfloat162 a = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+        return fmaxf(fmaxf(__low2float(a), __high2float(a)), 0.0f);   // (0: all are NaN)
+    }
+    float v[8], m = 0.0f;
+    values8(r, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
     return m;
@@ -70,21 +103,51 @@ __device__ __forceinline__ void store_codes8(uint8_t *dst, int64_t c, int64_t W,
         if (c + j < W) dst[j] = (uint8_t)((j < 4 ? q.x >> (8 * j) : q.y >> (8 * (j - 4))) & 0xffu);
 }
 
-// One scale for 128 values of a row.
+// The blocks of 128 values of the rows of [outer, H, W], sixteen lanes each, two a warp, are dealt out to the warps round by round. Which matrix, row and block a
+// lane's next one is follows from the last one's by additions (64-bit divisions for each cost as much as its codes). The launchers keep the blocks below 2^31.
+struct RowWalk {
+    uint32_t i, b, h, o, step, step_b, step_h, step_o, total, blocks, H;
+    __device__ RowWalk(int64_t rows, int64_t H_, int64_t W) : total((uint32_t)(rows * f8_blocks(W))), blocks((uint32_t)f8_blocks(W)), H((uint32_t)H_) {
+        step = gridDim.x * 16;
+        i = blockIdx.x * 16 + (threadIdx.x >> 4);
+        split(i, b, h, o);
+        split(step, step_b, step_h, step_o);
+    }
+    __device__ void split(uint32_t x, uint32_t &block, uint32_t &in, uint32_t &out) const {
+        const uint32_t row = x / blocks;
+        block = x - row * blocks;
+        out = row / H;
+        in = row - out * H;
+    }
+    __device__ bool here() const { return i < total; }
+    __device__ bool warp_here() const { return i - ((threadIdx.x >> 4) & 1) < total; }   // (all lanes of a warp take part in the shuffles)
+    __device__ void next() {
+        i += step;
+        b += step_b;
+        h += step_h;
+        o += step_o;
+        if (b >= blocks) { b -= blocks; ++h; }
+        if (h >= H) { h -= H; ++o; }
+    }
+};
+
+// One scale for 128 values of a row. The values of the next block are on their way while this one's codes are made.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(Source src, uint8_t *codes, float *scales, int64_t rows, int64_t H, int64_t W, bool vector_out) {
-    const int64_t blocks = f8_blocks(W);
+__global__ void __launch_bounds__(256, 6) quantize_rows_kernel(Source src, uint8_t *codes, float *scales, int64_t rows, int64_t H, int64_t W, bool vector_out) {
     const int sub = threadIdx.x & 15;
-    // (all lanes of a warp take part in the shuffles)
-    const int64_t total = rows * blocks, step = (int64_t)gridDim.x * 16;
-    for (int64_t first = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 5) * 2; first < total; first += step) {
-        const int64_t i = first + ((threadIdx.x >> 4) & 1);
-        const int64_t r = i / blocks, b = i - r * blocks, o = r / H;
-        const int64_t c = b * kF8Block + sub * 8;
-        float v[8] = {};
-        if (i < total) load8<T>(src, o, r - o * H, c, W, v);
-        const float scale = f8_scale(amax16lanes(amax8(v)));
-        if (i < total) {
+    RowWalk at(rows, H, W);
+    auto load = [&]() { return at.here() ? load8<T>(src, at.o, at.h, (int64_t)at.b * kF8Block + sub * 8, W) : Raw8<T>{}; };
+    Raw8<T> raw = load();
+    while (at.warp_here()) {
+        const uint32_t i = at.i;
+        const int64_t r = (int64_t)at.o * H + at.h, c = (int64_t)at.b * kF8Block + sub * 8;
+        float v[8];
+        values8(raw, v);
+        const float m = amax8(raw);
+        at.next();
+        raw = load();
+        const float scale = f8_scale(amax16lanes(m));
+        if (i < at.total) {
             store_codes8(codes + r * W + c, c, W, f8_pack8(v, scale), vector_out);
             if (sub == 0) scales[i] = scale;
         }
@@ -93,24 +156,28 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(Source src, uint8_t 
 
 // One scale for a block of 128 x 128: a thread block each, 32 values a thread. (256 threads with 64 values, 100 registers, took 30 us for 4096 x 4096 fp32.)
 template <typename T>
-__global__ void __launch_bounds__(512, 2) quantize_blocks_kernel(Source src, uint8_t *codes, float *scales, int64_t H, int64_t W, bool vector_out) {
+__global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : 3) quantize_blocks_kernel(Source src, uint8_t *codes, float *scales, int64_t H, int64_t W, bool vector_out) {
     __shared__ float red[16];
-    const int64_t wb = f8_blocks(W), hb = f8_blocks(H);
-    const int64_t i = blockIdx.x, o = i / (hb * wb), h0 = (i / wb % hb) * kF8Block, c = i % wb * kF8Block + (threadIdx.x & 15) * 8;
+    const uint32_t wb = (uint32_t)f8_blocks(W), hb = (uint32_t)f8_blocks(H), i = blockIdx.x, row = i / wb;   // (the launcher keeps the blocks below 2^31)
+    const int64_t o = row / hb, h0 = (int64_t)(row - row / hb * hb) * kF8Block, c = (int64_t)(i - row * wb) * kF8Block + (threadIdx.x & 15) * 8;
     const int r0 = threadIdx.x >> 4;
-    float v[4][8], m = 0.0f;
+    Raw8<T> raw[4];
+    float m = 0.0f;
+    if (src.vector && h0 + kF8Block <= H && c + 8 <= W) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t r = h0 + r0 + 32 * j;
-        if (r < H) {
-            load8<T>(src, o, r, c, W, v[j]);
-        } else {
+        for (int j = 0; j < 4; ++j) raw[j] = load8<T>(src, o, h0 + r0 + 32 * j, c);
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = h0 + r0 + 32 * j;
+            const Raw8<T> x = r < H ? load8<T>(src, o, r, c, W) : Raw8<T>{};
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[j][q] = 0.0f;
+            for (int q = 0; q < 4; ++q)
+                if (q == j) raw[q] = x;
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, amax8(v[j]));
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, amax8(raw[j]));
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -122,28 +189,33 @@ __global__ void __launch_bounds__(512, 2) quantize_blocks_kernel(Source src, uin
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int64_t r = h0 + r0 + 32 * j;
-        if (r < H) store_codes8(codes + (o * H + r) * W + c, c, W, f8_pack8(v[j], scale), vector_out);
+        float v[8];
+        values8(raw[j], v);
+        if (r < H) store_codes8(codes + (o * H + r) * W + c, c, W, f8_pack8(v, scale), vector_out);
     }
     if (threadIdx.x == 0) scales[i] = scale;
 }
 
 // Activations into the operand layout. Without `pos` row r goes to row r; with it to the rows pos[r * k + j] (-1: nowhere).
-__global__ void __launch_bounds__(256) quantize_operand_kernel(Source src, int64_t rows, int64_t H, int64_t K, F8Activation out, const int32_t *pos, int k,
+__global__ void __launch_bounds__(256, 6) quantize_operand_kernel(Source src, int64_t rows, int64_t H, int64_t K, F8Activation out, const int32_t *pos, int k,
                                                                bool early) {
     if (early) ptx::grid_dep_launch();
     ptx::grid_dep_wait();
     if (!early) ptx::grid_dep_launch();
-    const int64_t blocks = f8_blocks(K);
     const int sub = threadIdx.x & 15;
-    const int64_t total = rows * blocks, step = (int64_t)gridDim.x * 16;
-    for (int64_t first = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 5) * 2; first < total; first += step) {
-        const int64_t i = first + ((threadIdx.x >> 4) & 1);
-        const int64_t r = i / blocks, b = i - r * blocks, o = r / H;
-        const int64_t c = b * kF8Block + sub * 8;
-        float v[8] = {};
-        if (i < total) load8<uint16_t>(src, o, r - o * H, c, K, v);
-        const float scale = f8_scale(amax16lanes(amax8(v)));
-        if (i >= total) continue;
+    RowWalk at(rows, H, K);
+    auto load = [&]() { return at.here() ? load8<uint16_t>(src, at.o, at.h, (int64_t)at.b * kF8Block + sub * 8, K) : Raw8<uint16_t>{}; };
+    Raw8<uint16_t> raw = load();
+    while (at.warp_here()) {
+        const uint32_t i = at.i;
+        const int64_t r = (int64_t)at.o * H + at.h, b = at.b;
+        float v[8];
+        values8(raw, v);
+        const float m = amax8(raw);
+        at.next();
+        raw = load();
+        const float scale = f8_scale(amax16lanes(m));
+        if (i >= at.total) continue;
         const uint2 q = f8_pack8(v, scale);
         for (int j = 0; j < k; ++j) {
             const int64_t to = pos ? pos[r * k + j] : r;
@@ -170,7 +242,7 @@ int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, in
                                 bool early, cudaStream_t stream) {
     const int64_t rows = outer * H, want = (rows * f8_blocks(K) + 15) / 16;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(want < 148 * 8 ? (want > 0 ? want : 1) : 148 * 8));
+    cfg.gridDim = dim3((unsigned)(want < 148 * 6 ? (want > 0 ? want : 1) : 148 * 6));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -200,9 +272,10 @@ extern "C" int32_t ttb_quantize_float8(const void *src, int32_t src_dtype, int32
         return fail(TTB_E_INVALID, "ttb_quantize_float8: misaligned pointer");
     const ttb::Source s = ttb::make_source(src, src_dtype, src_row_major != 0, H, W);
     const bool vector_out = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && W % 8 == 0;
+    if (outer * H > INT32_MAX || outer * H * ttb::f8_blocks(W) > INT32_MAX) return fail(TTB_E_UNSUPPORTED, "ttb_quantize_float8: too many blocks");
     if (block_rows == 1) {
         const int64_t want = (outer * H * ttb::f8_blocks(W) + 15) / 16;
-        const unsigned grid = (unsigned)(want < 148 * 64 ? want : 148 * 64);
+        const unsigned grid = (unsigned)(want < 148 * 6 ? want : 148 * 6);
         auto kernel = src_dtype == TTB_FLOAT32 ? ttb::quantize_rows_kernel<float> : ttb::quantize_rows_kernel<uint16_t>;
         kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(s, (uint8_t *)codes, (float *)scales, outer * H, H, W, vector_out);
     } else {
