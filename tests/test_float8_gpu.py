@@ -55,6 +55,24 @@ def test_quantize_equals_the_definition(dev, shape, rows, dtype, layout):
 
 
 @pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_at_every_magnitude(dev, rows, dtype):
+    """Quotients are those of a division from the smallest numbers to the largest, zeros of either sign among them, next to borders between two codes too."""
+    exponents = torch.arange(-148, 127, 2, dtype=torch.float64)
+    x = torch.randn(exponents.numel(), 128, 128, generator=gen(17), dtype=torch.float64).clamp(-3.9, 3.9) * torch.exp2(-10 * torch.rand(128, 128, generator=gen(18), dtype=torch.float64))
+    x[:, 0, :] = torch.tensor([448.0, 17.0, 19.0, -21.0, 23.0, 25.0, 27.0, -29.0]).repeat(16) / 448 * 3.5
+    x = (x * torch.exp2(exponents)[:, None, None]).float()
+    x[:, 1] = torch.nextafter(x[:, 0], torch.tensor(math.inf))
+    x[:, 2] = torch.nextafter(x[:, 0], torch.tensor(-math.inf))
+    x[:, 3, ::2] = -0.0
+    x = x.reshape(-1, 128).to(dtype)
+    q = ttnn.quantize_float8(put(x, dev), block_rows=rows)
+    codes, scales = ref.quantize(x, rows)
+    assert same_bits(ttnn.to_torch(q.scales), scales)
+    assert same_bits(ttnn.to_torch(q.codes), codes)
+
+
+@pytest.mark.parametrize("rows", [1, 128])
 def test_quantize_of_special_values(dev, rows):
     x = torch.zeros(128, 6 * 128)
     x[:, 0:128] = 0.0
@@ -404,6 +422,15 @@ def test_route_of_not_a_number_and_infinity(dev):
     bias[e[0, 0]] = -math.inf                     # an expert switched off
     e2 = ttnn.to_torch(ttnn.route_to_experts(put(x[:1], dev), 3, bias=put(bias, dev))[1])
     assert int(e[0, 0]) not in e2[0].tolist()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_infinity_by_score(dev, score):
+    x = torch.randn(3, 40, generator=gen(13))
+    x[0, 9] = x[0, 20] = x[2, 39] = math.inf
+    w, e = (ttnn.to_torch(t) for t in ttnn.route_to_experts(put(x, dev), 3, score=score, bias=put(torch.zeros(40), dev)))
+    assert e[0, :2].tolist() == [9, 20] and e[2, 0] == 39 and (e < 40).all()
+    assert torch.isnan(w[[0, 2]]).all() == (score == "softmax") and torch.isfinite(w[1]).all()
 
 
 def test_route_vanishing_scores(dev):

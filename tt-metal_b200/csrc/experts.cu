@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
         if (e < p.E) {
             const int64_t at = p.row_major ? r * p.E + e : o * (((p.H + 31) & ~(int64_t)31) * ((p.E + 31) & ~31)) + tiled_offset(h, e, (p.E + 31) >> 5);
             x[i] = p.bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p.logits)[at] << 16) : reinterpret_cast<const float *>(p.logits)[at];
-            nan |= x[i] != x[i];
+            nan |= x[i] != x[i] || (x[i] == CUDART_INF_F && !p.sigmoid);   // (inf - inf in the softmax)
             most = fmaxf(most, x[i]);
         }
     }
@@ -156,6 +156,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
     most = from_ordered(__reduce_max_sync(0xffffffffu, ordered(most)));
     const bool by_score = p.bias != nullptr || (p.groups > 1 && p.sum_of_two);
     double *const mine = choice_smem + (size_t)warp * p.E;
+    // exp's argument; among infinite logits, whose softmax is NaN, those come first all the same
+    auto below = [&](auto v) { return v == most ? decltype(v)(0) : v - decltype(v)(most); };
     auto is_free = [&](int i) { return i * 32 + lane < p.E && x[i] > -CUDART_INF_F; };   // (false for a NaN)
     int my_id;
     float my_x, first, key[V];
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
             total = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (is_free(i)) total += expf(x[i] - most);
+                if (is_free(i)) total += expf(below(x[i]));
 #pragma unroll
             for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
         }
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
         for (int i = 0; i < V; ++i) {
             key[i] = -CUDART_INF_F;
             if (is_free(i)) {
-                const float s = p.sigmoid ? 1.0f / (1.0f + expf(-x[i])) : expf(x[i] - most) / total, b = p.bias ? p.bias[i * 32 + lane] : 0.0f;
+                const float s = p.sigmoid ? 1.0f / (1.0f + expf(-x[i])) : expf(below(x[i])) / total, b = p.bias ? p.bias[i * 32 + lane] : 0.0f;
                 key[i] = s + b == s + b ? s + b : -CUDART_INF_F;
                 if (fabsf(b) < CUDART_INF_F) size = fmaxf(size, fabsf(b));
             }
@@ -192,11 +194,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
         total = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (is_free(i)) total += exp((double)x[i] - (double)most);
+            if (is_free(i)) total += exp(below((double)x[i]));
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     }
-    auto score = [&](float v) { return p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)most) / total; };
+    auto score = [&](float v) { return p.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp(below((double)v)) / total; };
     if (!sure) {   // two values next to each other: again in 64 bits
         double key64[V];
 #pragma unroll

@@ -149,7 +149,7 @@ Routing route_to_experts(const Tensor &logits, int k, const std::string &score, 
     Device *dev = logits.device();
     dev->make_current();
     std::vector<int64_t> od = logits.shape().dims();
-    od.back() = std::max(k, 1);
+    od.back() = std::clamp(k, 1, 32);   // (the call refuses others)
     const Shape shape(od);
     Routing r{Tensor(allocate_device_buffer(dev, physical_bytes(shape, DataType::FLOAT32, Layout::ROW_MAJOR)), shape, DataType::FLOAT32, Layout::ROW_MAJOR),
               Tensor(allocate_device_buffer(dev, physical_bytes(shape, DataType::UINT32, Layout::ROW_MAJOR)), shape, DataType::UINT32, Layout::ROW_MAJOR)};

@@ -54,7 +54,8 @@ def route_to_experts(logits, k: int, *, score: str = "softmax", bias=None, group
     lowest index; with groups > 1 only among the top_groups groups of E / groups neighbouring experts whose best expert (group_score "max") or two best
     together ("top2_sum") count most. Weights are the chosen experts' scores (without bias) times `scale`, divided by their sum under `renormalize`.
     The order is that of 64-bit values. An expert whose logit is -inf is never chosen; where a row has too few left, the remaining places hold the index E
-    and the weight 0 (ttnn.experts_mlp_float8 skips them: a row of -inf gets no expert). A row with a NaN has NaN weights."""
+    and the weight 0 (ttnn.experts_mlp_float8 skips them: a row of -inf gets no expert). The experts of a row with a NaN, or an infinity
+    under softmax, have NaN weights; a NaN's own is never chosen."""
     weights, experts = _ttnn.route_to_experts(_unwrap(logits), k, score=score, bias=_unwrap(bias) if bias is not None else None, groups=groups,
                                               top_groups=top_groups, group_score=group_score, renormalize=renormalize, scale=scale)
     return _wrap(logits, weights), _wrap(logits, experts)
