@@ -14,7 +14,7 @@
 // The blocks that share a tile leave their fp32 sums in scratch and take a ticket; the last one adds them in block order (so results
 // repeat bit for bit) and finishes the rows. No block waits for another. A block's range ends with the first part of a tile, whose other parts are the
 // beginnings of other blocks' ranges: it mostly finds them all there and adds them to its sums in registers.
-// What bounds it (2048 x 8192 x 28672, 489 us in a graph, 1966 TFLOP/s): a block's copies, 48 KB for a unit of 128 x 256 x 128 or 61 B per clock and SM (331 us
+// What bounds it (2048 x 8192 x 28672, 477 us in a graph with the quantiser, 2017 TFLOP/s): a block's copies, 48 KB for a unit of 128 x 256 x 128 or 61 B per clock and SM (331 us
 // by themselves), with the MMAs 398, and the turns of an accumulator, of which two alternate. A tile's results take 3 us to store (fp32 6), and a unit 0.5.
 // Every mbarrier wait is bounded; a wait that runs out raises a status word instead of hanging.
 #include "float8_tiles.cuh"
