@@ -236,7 +236,7 @@ int32_t ttb_matmul_decode_static(const void *a_dev, int32_t a_dtype, const void 
  * ttb_quantize_float8: src [outer, H, W] (TTB_FLOAT32 or TTB_BFLOAT16, tiled or row-major) -> codes row-major [outer, H, W], one byte
  * each, and scales [outer, ceil(H / block_rows), ceil(W / 128)], block_rows 1 or 128:
  *   scale = max(largest magnitude of the block, 2^-100) / 448, code = x / scale, both quotients rounded to fp32 and the code then to the nearest
- * e4m3 number, ties to even. A NaN becomes the NaN code and does not count for the scale; a block with an infinity gets the scale inf. */
+ * e4m3 number, ties to even. A NaN becomes the NaN code and does not count for the scale; a block with an infinity gets the scale inf. Up to 2^31 - 1 rows and as many blocks (TTB_E_UNSUPPORTED behind that). */
 int32_t ttb_quantize_float8(const void *src_dev, int32_t src_dtype, int32_t src_row_major, void *codes_dev, void *scales_dev, int64_t outer, int64_t H,
                             int64_t W, int32_t block_rows, void *stream);
 /* out[rows, N] = act( q(a)[rows, K] x w^T + bias ), fp32 accumulation: `a` (bfloat16) is quantised with block_rows 1; w_codes [N, K] and w_scales

@@ -48,7 +48,8 @@ def test_quantize_refusals():
     _says(c, call(rows=64), INVALID, "block_rows")
     for kw in ({"outer": 0}, {"h": 0}, {"w": -1}):
         _says(c, call(**kw), INVALID, "positive")
-    for kw in ({"h": 1 << 41}, {"outer": 1 << 20, "h": 1 << 20, "w": 2}, {"outer": 1 << 62, "h": 4}):
+    for kw in ({"h": 1 << 41}, {"outer": 1 << 20, "h": 1 << 20, "w": 2}, {"outer": 1 << 62, "h": 4}, {"h": 1 << 31, "w": 1}, {"h": 1 << 31, "w": 1, "rows": 1},
+               {"h": 1 << 30, "w": 300, "rows": 1}):
         _says(c, call(**kw), UNSUPPORTED, "too many")
     _says(c, call(src=A + 2), INVALID, "misaligned")
     _says(c, call(dtype=0, src=A + 1), INVALID, "misaligned")

@@ -102,6 +102,21 @@ def test_quantize_of_special_values(dev, rows):
     assert hit == math.inf and torch.isnan(codes[7, 530]) and (codes[7, 531:640] == 0).all()
 
 
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("layout", [ttnn.ROW_MAJOR_LAYOUT, ttnn.TILE_LAYOUT])
+def test_quantize_bfloat16_rows_with_nan(dev, rows, layout):
+    x = torch.randn(128, 384, generator=gen(19)).bfloat16()
+    hole = torch.rand(128, 384, generator=gen(20)) < 0.3
+    hole[:, 128:256] = True                           # nothing but NaN
+    clean = x.masked_fill(hole, 0.0)
+    x[hole] = math.nan
+    q = ttnn.quantize_float8(put(x, dev, layout), block_rows=rows)
+    codes, scales = ref.quantize(clean, rows)
+    got = ttnn.to_torch(q.codes).float()
+    assert same_bits(ttnn.to_torch(q.scales), scales)
+    assert torch.equal(got.isnan(), hole) and torch.equal(got[~hole], codes.float()[~hole])
+
+
 # ---- linear ----------------------------------------------------------------------------------------------------------------
 LINEAR = [(1, 16, 1), (1, 128, 128), (1, 4096, 1024), (2, 144, 130), (7, 256, 8), (8, 400, 129), (9, 2048, 264), (31, 4544, 96), (33, 1024, 1000), (64, 512, 2048),
           (100, 8192, 136), (128, 128, 256), (129, 272, 257), (200, 1024, 512), (257, 640, 384), (350, 4544, 4672), (1025, 256, 520), (2500, 144, 130), (512, 2048, 2048)]
