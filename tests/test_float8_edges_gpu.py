@@ -1,0 +1,50 @@
+"""float8 operators where their contract is easy to miss: codes of the experts' inner quantisation, rows that are not finite under activations and in the
+padding of tiled results, saturated router scores."""
+import math
+
+import pytest
+import torch
+
+import cabi
+import float8_ref as ref
+import ttnn
+from test_float8_gpu import dev, no_wait_ran_out, pair, put, same_bits  # noqa: F401  (fixtures among them)
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- the experts' inner quantisation ---------------------------------------------------------------------------------------
+def _products():
+    """Gate and up codes [256, 127] whose products are exact in 32 bits, and their quotients' codes by division and by a rounded reciprocal."""
+    g = gen(1)
+    gate, up = ((torch.randn(256, 127, generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in range(2))
+    h = (gate.float() * up.float()).T.contiguous()
+    codes, scales = ref.quantize(h, 1)
+    by_reciprocal = (h * ref.spread(torch.ones_like(scales) / scales, 1, *h.shape)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    differ = (codes.view(torch.uint8) != by_reciprocal.view(torch.uint8)).any(1)
+    order = torch.argsort(differ.int(), descending=True, stable=True)   # the rows that tell the two apart first
+    return gate[:, order], up[:, order], h[order], int(differ.sum())
+
+
+@pytest.mark.parametrize("rows", [3, 20, 50, 100])
+@pytest.mark.parametrize("act", [None, "relu"])
+def test_experts_inner_codes_are_those_of_the_quantiser(dev, rows, act):
+    """Every number up to the quantisation is exact (a row of x picks a column of the weights), the down weight is a unit matrix: the result is code * scale."""
+    gate, up, h, telling = _products()
+    assert telling >= 3
+    x = torch.zeros(rows, 256)
+    x[torch.arange(rows), torch.arange(rows)] = 256.0   # a code of its own, as the row's scale is 1:
+    x[:, 127] = 448.0
+    wide = [torch.cat([w.view(torch.uint8), torch.zeros(256, 129, dtype=torch.uint8)], 1).view(torch.float8_e4m3fn)[None] for w in (gate, up)]
+    scale = torch.full((1, 2, 2), 2.0 ** -8)
+    down = torch.eye(256)[None].to(torch.float8_e4m3fn), torch.ones(1, 2, 2)
+    ids, p = torch.zeros(rows, 1, dtype=torch.int32), torch.ones(rows, 1)
+    y = ttnn.experts_mlp_float8(put(x.bfloat16(), dev), put(ids, dev), put(p, dev), pair((wide[0], scale), dev), pair((wide[1], scale), dev), pair(down, dev), activation=act)
+    h = h[:rows] if act is None else torch.relu(gate.float().T[:rows]) * up.float().T[:rows]
+    codes, scales = ref.quantize(h, 1)
+    want = (codes.float() * ref.spread(scales, 1, *h.shape)).bfloat16()
+    assert torch.equal(ttnn.to_torch(y).float(), want.float())

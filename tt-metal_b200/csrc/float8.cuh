@@ -40,29 +40,27 @@ __device__ __forceinline__ uint64_t f8_quotient2(uint64_t nx, uint64_t d, uint64
 }
 __device__ __forceinline__ float f8_scale(float amax) { return __fdiv_rn(fmaxf(amax, 0x1p-100f), 448.0f); }
 
-// Eight values as codes, the first in the lowest byte.
-__device__ __forceinline__ uint2 f8_pack8(const float (&x)[8], float scale) {
-    const bool small = scale < 0x1p-60f;   // (for the remainders; the quotients stay)
-    if (small) scale *= 0x1p64f;
-    const float inverse = __frcp_rn(scale), divisor = scale < CUDART_INF_F ? scale : 0.0f;   // scale inf: 0 for the finite values, else NaN
-    const uint64_t d = f8_two(divisor, divisor), ny = f8_two(-inverse, -inverse);
-    uint32_t h[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint64_t nx = f8_two(-x[2 * j], -x[2 * j + 1]);
+// Codes of the values of one block: what their quotients by its scale have in common, and four of them, the first in the lowest byte.
+struct F8Codes {
+    uint64_t d, ny;
+    bool small;   // (for the remainders; the quotients stay)
+    __device__ __forceinline__ explicit F8Codes(float scale) : small(scale < 0x1p-60f) {
+        if (small) scale *= 0x1p64f;
+        const float inverse = __frcp_rn(scale), divisor = scale < CUDART_INF_F ? scale : 0.0f;   // scale inf: 0 for the finite values, else NaN
+        d = f8_two(divisor, divisor);
+        ny = f8_two(-inverse, -inverse);
+    }
+    __device__ __forceinline__ uint32_t two(float x0, float x1) const {
+        uint64_t nx = f8_two(-x0, -x1);
         if (small) nx = f8_mul2(nx, f8_two(0x1p64f, 0x1p64f));
         const uint64_t q = f8_quotient2(nx, d, ny);
-        h[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float((uint32_t)q), __uint_as_float((uint32_t)(q >> 32))), __NV_SATFINITE, __NV_E4M3);
+        return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float((uint32_t)q), __uint_as_float((uint32_t)(q >> 32))), __NV_SATFINITE, __NV_E4M3);
     }
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-}
-
-// The same with the scale's reciprocal, for values that are rounded sums themselves: a quotient that this moves by a unit in the last place was as uncertain
-// before, and the divisions of a tile are some 20 KB of code.
-__device__ __forceinline__ uint32_t f8_pack4_by(const float *v, float inverse) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inverse, v[1] * inverse), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inverse, v[3] * inverse), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+    __device__ __forceinline__ uint32_t four(const float *x) const { return two(x[0], x[1]) | (two(x[2], x[3]) << 16); }
+};
+__device__ __forceinline__ uint2 f8_pack8(const float (&x)[8], float scale) {
+    const F8Codes codes(scale);
+    return make_uint2(codes.four(x), codes.four(x + 4));
 }
 
 // Quantised activations in scratch: for every block of 128 columns all rows, 128 bytes each, with the 16-byte chunks of a row

@@ -392,10 +392,11 @@ __device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n
     }
 }
 
-// act(g) * u; silu with the fast division (2 units in the last place; 0 where the exponential leaves its range, as it should be).
+// act(g) * u; silu with a division that is right to 2 units in the last place, like the exponential (where 1 + exp(-g) passes 2^126 the result, less than 2^-119 of u,
+// becomes 0). The fast exponential would be off by a part of 2^-24 that grows with |g|.
 template <int ACT>
 __device__ __forceinline__ float gate(float g, float u) {
-    if (ACT == TTB_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g)) * u;
+    if (ACT == TTB_ACT_SILU) return __fdividef(g, 1.0f + expf(-g)) * u;
     return apply_activation_t<ACT>(g) * u;
 }
 
@@ -411,13 +412,14 @@ __device__ __forceinline__ bool finish_gated(const Args &p, int row, bool valid,
     }
     red[part][lane_row] = m;
     if (!meet(p)) return false;
-    const float scale = f8_scale(fmaxf(m, red[part ^ 1][lane_row])), inverse = __frcp_rn(scale);
+    const float scale = f8_scale(fmaxf(m, red[part ^ 1][lane_row]));
     if (!meet(p)) return false;   // (the next tile writes `red` again)
     if (!valid) return true;
+    const F8Codes codes(scale);
 #pragma unroll
     for (int q = 0; q < 64; q += 16)
         *reinterpret_cast<uint4 *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, part * 64 + q)) =
-            make_uint4(f8_pack4_by(acc + q, inverse), f8_pack4_by(acc + q + 4, inverse), f8_pack4_by(acc + q + 8, inverse), f8_pack4_by(acc + q + 12, inverse));
+            make_uint4(codes.four(acc + q), codes.four(acc + q + 4), codes.four(acc + q + 8), codes.four(acc + q + 12));
     if (part == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
     return true;
 }
@@ -460,7 +462,7 @@ __device__ __forceinline__ void finish_row_warp(const Args &p, int row, int c, i
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         const float scale = f8_scale(m);
-        *reinterpret_cast<uint32_t *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, lane * 4)) = f8_pack4_by(h, __frcp_rn(scale));
+        *reinterpret_cast<uint32_t *>(p.h.codes + f8_act_offset(p.h.rows_padded, c, row, lane * 4)) = F8Codes(scale).four(h);
         if (lane == 0) p.h.scales[row * p.h.scale_pitch + c] = scale;
     } else {
 #pragma unroll
