@@ -243,8 +243,9 @@ int32_t ttb_quantize_float8(const void *src_dev, int32_t src_dtype, int32_t src_
  * [ceil(N / 128), ceil(K / 128)] as ttb_quantize_float8 leaves them with block_rows 128 (any positive scales serve). K is a multiple of 16, rows and N are
  * free; tiled tensors have a multiple of 32 rows, and their columns behind N come out as zeros. `bias`: NULL, or bfloat16, the first row of a tiled [32, N]
  * (TTB_MM_BIAS_ROW_MAJOR: [N]). `out`: TTB_BFLOAT16 or TTB_FLOAT32. Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR, TTB_MM_BIAS_ROW_MAJOR and, as for ttb_matmul,
- * with whose calls a workspace can be shared, TTB_MM_WORKSPACE_ZEROED (else the counters at its head are cleared with a memset) and TTB_MM_WEIGHTS_RESIDENT. The
- * workspace is touched between launch and completion on `stream`. Results repeat bit for bit. */
+ * with whose calls a workspace can be shared, TTB_MM_WORKSPACE_ZEROED (else the counters at its head are cleared with a memset) and TTB_MM_WEIGHTS_RESIDENT
+ * (not for the call right behind the one that wrote the codes, ttb_quantize_float8 included). The workspace
+ * is touched between launch and completion on `stream`. Results repeat bit for bit. */
 int64_t ttb_linear_float8_workspace_bytes(int64_t rows, int64_t K, int64_t N);
 int32_t ttb_linear_float8(const void *a_dev, const void *w_codes_dev, const void *w_scales_dev, const void *bias_dev, void *out_dev, int32_t out_dtype,
                           int64_t rows, int64_t K, int64_t N, int32_t activation, int32_t flags, void *workspace_dev, int64_t workspace_bytes, void *stream);

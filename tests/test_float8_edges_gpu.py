@@ -48,3 +48,20 @@ def test_experts_inner_codes_are_those_of_the_quantiser(dev, rows, act):
     codes, scales = ref.quantize(h, 1)
     want = (codes.float() * ref.spread(scales, 1, *h.shape)).bfloat16()
     assert torch.equal(ttnn.to_torch(y).float(), want.float())
+
+
+# ---- calls right behind the one that writes their weight -------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 5, 40, 200])
+def test_linear_right_behind_its_weights_quantiser(dev, rows):
+    """Nothing between the two calls; the codes lie where another weight's were the call before."""
+    g = gen(4)
+    n, k = 2048, 4096
+    x = ref.rows_of(g, rows, k)
+    ws = [torch.randn(n, k, generator=g) * s for s in (0.02, 0.5, 0.001)]
+    xt, wts = put(x, dev), [put(w, dev) for w in ws]
+    want = [ref.linear(x.cuda(), *(t.cuda() for t in ref.quantize(w, 128)), None, None, torch.bfloat16) for w in ws]
+    for turn in range(6):
+        q = ttnn.quantize_float8(wts[turn % 3])
+        y = ttnn.linear_float8(xt, q)
+        del q
+        ref.assert_within(ttnn.to_torch(y), *want[turn % 3], turn)

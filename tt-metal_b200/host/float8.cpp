@@ -121,9 +121,10 @@ Tensor linear_float8(const Tensor &x, const Float8 &w, const std::optional<Tenso
     auto outb = allocate_device_buffer(dev, physical_bytes(out_shape, out_dtype, x.layout()));
     const int64_t need = ttb_linear_float8_workspace_bytes(rows, K, N);
     void *ws = need > 0 ? dev->workspace(need) : nullptr;
-    // A float8 weight is written by a copy or by the quantiser, which lets no later kernel start before it has ended: it is complete before any kernel that this one may overlap.
+    // Not TTB_MM_WEIGHTS_RESIDENT: the operation before may be the one that writes the codes (ttnn.quantize_float8, or whatever fills memory that this API only wraps),
+    // and a kernel that starts early sees its stores only after waiting for it.
     check(ttb_linear_float8(x.data(), w.codes.data(), w.scales.data(), bias_ptr, outb->ptr, static_cast<int>(out_dtype), rows, K, N, act,
-                            flags | TTB_MM_WORKSPACE_ZEROED | TTB_MM_WEIGHTS_RESIDENT, ws, need, nullptr),
+                            flags | TTB_MM_WORKSPACE_ZEROED, ws, need, nullptr),
           op);
     return Tensor(outb, out_shape, out_dtype, x.layout());
 }
