@@ -65,3 +65,43 @@ def test_linear_right_behind_its_weights_quantiser(dev, rows):
         y = ttnn.linear_float8(xt, q)
         del q
         ref.assert_within(ttnn.to_torch(y), *want[turn % 3], turn)
+
+
+# ---- waits that are bounded ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,k,n", [(5120, 8192, 28672), (32, 8192, 148 * 15 * 256 + 50 * 256), (64, 8192, 148 * 15 * 256 + 50 * 256)])
+def test_a_launch_longer_than_the_wait_limit_is_no_timeout(rows, k, n):
+    """Rounds of whole tiles that take longer than the shortest limit, about half a millisecond, and then 40 to 50 tiles that several blocks share, most blocks two of
+    them. The limit is for a step of a launch, not for all of it."""
+    c = ref.lib()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    codes = torch.empty(n, k, dtype=torch.float8_e4m3fn, device="cuda")
+    for part in codes.split(16384):
+        part.copy_((torch.randn(part.shape, generator=g, device="cuda") * 100).clamp_(-448, 448))
+    scales = (torch.rand(ref.blocks(n), ref.blocks(k), generator=g, device="cuda") + 0.5) * (2.0 / 100 / k ** 0.5)
+    x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    out = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    need = c.ttb_linear_float8_workspace_bytes(rows, k, n)
+    space = torch.zeros(need, dtype=torch.uint8, device="cuda")
+
+    def call():
+        assert c.ttb_linear_float8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), None, out.data_ptr(), 0, rows, k, n, 0, 3 | cabi.MM_WORKSPACE_ZEROED, space.data_ptr(), need,
+                                   torch.cuda.current_stream().cuda_stream) == 0
+    call()
+    lib = cabi.load()
+    lib.check(lib.set_wait_limit_cycles(1))
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    try:
+        start.record()
+        call()
+        end.record()
+        torch.cuda.synchronize()
+    finally:
+        lib.check(lib.set_wait_limit_cycles(0))
+    assert lib.check_status(None) == 0
+    assert start.elapsed_time(end) > 0.6
+    pick = torch.cat([torch.arange(0, n, n // 37, device="cuda"), torch.arange(n - 130, n, device="cuda")])   # (the shared tiles come last)
+    few = torch.arange(0, rows, max(1, rows // 40), device="cuda")
+    w = codes[pick].double() * scales.double()[pick // 128].repeat_interleave(128, 1)
+    want, tol = ref.sums(ref.requantized(x[few]), w)
+    ref.assert_within(out[few][:, pick], want, tol + (want.abs() + tol) * 2.0 ** -8, (rows, n))
+    assert int(space[:65536].count_nonzero()) == 0

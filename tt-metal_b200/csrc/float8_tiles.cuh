@@ -529,17 +529,39 @@ __device__ __forceinline__ void add_parts(const Args &p, F part_of, int c0, int 
     }
 }
 
+// mbar_wait for what lies any number of units ahead: the limit is for the time without progress, the number of the unit that the adding warps are at. (A wait with
+// one limit for all of it would run out in a sound launch that is longer than the limit.)
+__device__ __forceinline__ bool wait_while_units_pass(uint32_t bar, uint32_t parity, volatile int *progress, volatile int *abort_flag, int *status, int code, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    int at = *progress;
+    long long t0 = clock64();
+    for (uint32_t spin = 1;; ++spin) {
+        if (mbar_try_wait_suspend(bar, parity, 4000u)) return true;
+        if ((spin & 7u) == 0u) {
+            if (*abort_flag) return false;
+            if (*progress != at) {
+                at = *progress;
+                t0 = clock64();
+            } else if (clock64() - t0 > limit) {
+                *abort_flag = 1;
+                atomicCAS(status, 0, code);
+                return false;
+            }
+        }
+    }
+}
+
 // The warp that takes the ticket for the one shared tile that is not its block's last segment (a range is at most a tile long), while the next segment runs:
 // `handed` says that its part is written. Where all parts are there with it, it finishes the tile itself if it has few rows (ADD), else the adding warps do it after
 // their last segment (`pending`: the tile, or -1; then `told`): one warp alone took 126 x 18272 x 6376 from 47 to 83 us.
 template <int ACT, int W, bool GATED, bool ADD>
-__device__ __forceinline__ void hand_over(const Args &p, uint32_t handed, uint32_t told, volatile int *pending, volatile int *abort_flag, Walk walk, const int *off, const int *cum) {
+__device__ __forceinline__ void hand_over(const Args &p, uint32_t handed, uint32_t told, volatile int *pending, volatile int *progress, volatile int *abort_flag, Walk walk, const int *off, const int *cum) {
     grid_dep_wait();
     const int lane = threadIdx.x & 31;
     Segment seg;
     while (walk.next(seg)) {
         if (seg.kb1 - seg.kb0 == p.Kb || walk.u >= walk.u_end) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(handed, 0, abort_flag, p.status, 56, wait_clocks(p)))) return;
+        if (!__all_sync(0xffffffffu, wait_while_units_pass(handed, 0, progress, abort_flag, p.status, 56, wait_clocks(p)))) return;
         const Sharing sh(walk, seg);
         int last = 0;
         if (lane == 0) last = take_ticket(p.tickets + sh.q) == sh.c1 - sh.c0;

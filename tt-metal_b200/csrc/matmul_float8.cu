@@ -60,7 +60,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_word;
     __shared__ int tiles_word;
-    __shared__ volatile int ticket, pending;
+    __shared__ volatile int ticket, pending, progress;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint8_t *after = smem + p.stages * p.stage_bytes;
@@ -84,7 +84,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
         mbar_init(all_bar, kAddWarps);
         mbar_init(handed_bar, kAddWarps);
         mbar_init(told_bar, 1);
-        abort_word = 0;
+        abort_word = progress = 0;
         fence_mbar_init();
     }
     if (warp == kIssueWarp) {
@@ -114,7 +114,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
                     mma_e4m3_ss(tmem_base + (uint32_t)(buf * 128 * W), a + 2 * k, b + 2 * k, instr_desc_e4m3(BM, 128 * W), k > 0);
             });
         } else {
-            hand_over<ACT, W, GATED, false>(p, handed_bar, told_bar, &pending, abort_flag, walk, off, cum);
+            hand_over<ACT, W, GATED, false>(p, handed_bar, told_bar, &pending, &progress, abort_flag, walk, off, cum);
         }
     } else {
         if (W == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
@@ -170,6 +170,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
             for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
             for (int kb = now.kb0; kb < now.kb1; ++kb, ++n) {
                 const int buf = n % NB;
+                if (threadIdx.x == 0) progress = n;
                 const float x = (kb & 2) ? ((kb & 1) ? c.xa.w : c.xa.z) : ((kb & 1) ? c.xa.y : c.xa.x);
                 const float f0 = x * __shfl_sync(0xffffffffu, c.w0, kb & 31), f1 = GATED ? x * __shfl_sync(0xffffffffu, c.w1, kb & 31) : f0;
                 if ((kb & 3) == 3) {

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_word;
     __shared__ int tiles_word;
-    __shared__ volatile int ticket, pending;
+    __shared__ volatile int ticket, pending, progress;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *sums = reinterpret_cast<float *>(smem + p.stages * p.stage_bytes);   // [tile_rows][128 W]
     int *off = reinterpret_cast<int *>(sums + p.tile_rows * 128 * W);
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
         mbar_init(handed_bar, kEpiWarps);
         mbar_init(told_bar, 1);
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(ready0 + 8u * i, 1);
-        abort_word = 0;
+        abort_word = progress = 0;
         fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     } else if (QUANT && warp >= kQuantWarp0) {
         quantise(p, ring, smem, ready0, scales, walk, off, cum, warp - kQuantWarp0);
     } else if (warp >= kMmaWarp + kIssuers) {
-        hand_over<ACT, W, GATED, ADD>(p, handed_bar, told_bar, &pending, abort_flag, walk, off, cum);
+        hand_over<ACT, W, GATED, ADD>(p, handed_bar, told_bar, &pending, &progress, abort_flag, walk, off, cum);
     } else {
         grid_dep_wait();
         const int quad = warp & 3, half = warp >> 2;
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
             for (int j = 0; j < NR; ++j) acc[j] = 0.0f;
             for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
                 const int buf = n % NB;
+                if (threadIdx.x == 0) progress = n;
                 const float w = __shfl_sync(0xffffffffu, w0, kb & 31);
                 float f[NX];
                 if (QUANT) {
