@@ -105,3 +105,28 @@ def test_a_launch_longer_than_the_wait_limit_is_no_timeout(rows, k, n):
     want, tol = ref.sums(ref.requantized(x[few]), w)
     ref.assert_within(out[few][:, pick], want, tol + (want.abs() + tol) * 2.0 ** -8, (rows, n))
     assert int(space[:65536].count_nonzero()) == 0
+
+
+# ---- rows that are not finite ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(5, 256, 200), (30, 400, 130), (50, 8192, 256), (100, 256, 264), (90, 8192, 130)])
+def test_linear_keeps_nan_under_every_activation(dev, act, rows, k, n):
+    g = gen(2)
+    x, w = ref.rows_of(g, rows, k), pair(ref.weight(g, n, k), dev)
+    b = put(torch.randn(1, n, generator=g).bfloat16(), dev)
+    clean = ttnn.to_torch(ttnn.linear_float8(put(x, dev), w, bias=b, activation=act))
+    x[1, 7], x[4, k - 1] = math.nan, math.inf
+    y = ttnn.to_torch(ttnn.linear_float8(put(x, dev), w, bias=b, activation=act))
+    assert torch.isnan(y[[1, 4]]).all()
+    keep = [i for i in range(rows) if i not in (1, 4)]
+    assert same_bits(y[keep], clean[keep]) and torch.isfinite(clean).all()
+
+
+@pytest.mark.parametrize("rows", [3, 20, 50, 100])
+def test_experts_keep_nan_under_relu(dev, rows):
+    g = gen(6)
+    x = ref.rows_of(g, rows, 256)
+    x[1, 7], x[2, 200] = math.nan, math.inf
+    ws = [pair(ref.weight(g, 256, 256, (1,)), dev) for _ in range(3)]
+    y = ttnn.to_torch(ttnn.experts_mlp_float8(put(x, dev), put(torch.zeros(rows, 1, dtype=torch.int32), dev), put(torch.ones(rows, 1), dev), *ws, activation="relu"))
+    assert torch.isnan(y[[1, 2]]).all() and torch.isfinite(y[[i for i in range(rows) if i not in (1, 2)]]).all()

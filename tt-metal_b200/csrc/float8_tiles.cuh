@@ -361,6 +361,12 @@ __device__ __forceinline__ void store16(const Args &p, int64_t row, int64_t n, c
     }
 }
 
+// The activation. (apply_activation_t's relu makes a NaN zero: the other matmuls keep that.)
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+    return ACT == TTB_ACT_RELU ? (v <= 0.0f ? 0.0f : v) : apply_activation_t<ACT>(v);
+}
+
 // 16 columns from n on: bias, activation, store.
 template <int ACT>
 __device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, float *v) {
@@ -371,7 +377,7 @@ __device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, 
             if (n + j < p.N) v[j] += __uint_as_float((uint32_t)__ldg(b + j) << 16);
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = apply_activation_t<ACT>(v[j]);
+    for (int j = 0; j < 16; ++j) v[j] = activate<ACT>(v[j]);
     store16(p, row, n, v);
 }
 
@@ -397,7 +403,7 @@ __device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n
 template <int ACT>
 __device__ __forceinline__ float gate(float g, float u) {
     if (ACT == TTB_ACT_SILU) return __fdividef(g, 1.0f + expf(-g)) * u;
-    return apply_activation_t<ACT>(g) * u;
+    return activate<ACT>(g) * u;
 }
 
 // act(g) * u of one row's 64 columns from part * 64 on, quantised with the scale of all 128: the two warps of the rows exchange their largest magnitudes
@@ -437,7 +443,7 @@ __device__ __forceinline__ void finish4(const Args &p, int64_t row, int64_t n, f
             if (n + j < p.N) v[j] += __uint_as_float((uint32_t)b[j] << 16);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = apply_activation_t<ACT>(v[j]);
+    for (int j = 0; j < 4; ++j) v[j] = activate<ACT>(v[j]);
     const int64_t off = p.out_row_major ? row * p.N + n : tiled_offset(row, n, width >> 5);
     const bool f32 = p.out_dtype == TTB_FLOAT32;
     if (p.out_aligned >= 16 && n + 4 <= width) {
