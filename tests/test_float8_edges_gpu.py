@@ -130,3 +130,18 @@ def test_experts_keep_nan_under_relu(dev, rows):
     ws = [pair(ref.weight(g, 256, 256, (1,)), dev) for _ in range(3)]
     y = ttnn.to_torch(ttnn.experts_mlp_float8(put(x, dev), put(torch.zeros(rows, 1, dtype=torch.int32), dev), put(torch.ones(rows, 1), dev), *ws, activation="relu"))
     assert torch.isnan(y[[1, 2]]).all() and torch.isfinite(y[[i for i in range(rows) if i not in (1, 2)]]).all()
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,k,n", [(32, 256, 70), (32, 8192, 130), (64, 512, 513), (160, 1024, 150), (96, 8192, 257)])
+def test_linear_columns_that_only_pad_are_zero(dev, rows, k, n, dtype, act):
+    """... in rows of NaN and infinities too, whose products with the zeros behind the weight's last row are not zero."""
+    g = gen(3)
+    x, w = ref.rows_of(g, rows, k), pair(ref.weight(g, n, k), dev)
+    x[1, 7], x[20, k - 1], x[31] = math.nan, math.inf, -math.inf
+    for b in (None, put(torch.randn(1, n, generator=g).bfloat16(), dev, ttnn.TILE_LAYOUT)):
+        y = ttnn.linear_float8(put(x, dev, ttnn.TILE_LAYOUT), w, bias=b, activation=act, dtype=getattr(ttnn, dtype))
+        full = ttnn.to_torch(y.reshape(ttnn.Shape(list(y.shape.padded))))
+        assert full.shape[-1] > n and (full[:, n:] == 0).all()
+        assert torch.isfinite(full[[0, 2, 21, 30]]).all()

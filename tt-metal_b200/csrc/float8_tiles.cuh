@@ -378,6 +378,11 @@ __device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, 
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = activate<ACT>(v[j]);
+    if (n + 16 > p.N) {   // (columns that only pad a tile: a NaN or an infinity of the row times the zeros behind the weight's last row is a NaN)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (n + j >= p.N) v[j] = 0.0f;
+    }
     store16(p, row, n, v);
 }
 
@@ -443,7 +448,7 @@ __device__ __forceinline__ void finish4(const Args &p, int64_t row, int64_t n, f
             if (n + j < p.N) v[j] += __uint_as_float((uint32_t)b[j] << 16);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = activate<ACT>(v[j]);
+    for (int j = 0; j < 4; ++j) v[j] = n + j < p.N ? activate<ACT>(v[j]) : 0.0f;   // (as in finish16)
     const int64_t off = p.out_row_major ? row * p.N + n : tiled_offset(row, n, width >> 5);
     const bool f32 = p.out_dtype == TTB_FLOAT32;
     if (p.out_aligned >= 16 && n + 4 <= width) {
