@@ -584,6 +584,7 @@ __device__ __forceinline__ void hand_over(const Args &p, uint32_t handed, uint32
             return;
         }
         if (!__shfl_sync(0xffffffffu, last, 0)) return;
+        __syncwarp();   // what lane 0 acquired with its ticket, the parts, is ordered before the other lanes' reads by this, not by the shuffle
         if (lane == 0) p.tickets[sh.q] = 0;
         const Tile T = tile_of(p, off, cum, seg.tile);
         auto part_of = [&](int block) { return sh.part(p, block, p.partial_rows * 128 * W); };
