@@ -258,8 +258,10 @@ int32_t ttb_linear_float8(const void *a_dev, const void *w_codes_dev, const void
  * their weights, row-major [outer * H, k]: experts (uint32) and weights (float32), best first, ties to the lowest index.
  *   score = softmax or sigmoid of the logits; choice value = score + bias[e] (float32 [E]; NULL: the score); with groups > 1 only the top_groups groups of
  *   neighbouring experts count. weight = score * scale, divided by the sum of the chosen scores under `renormalize` (zero where that sum is zero).
- * Order and ties are those of 64-bit choice values. An expert with logit or bias -inf is never chosen; where too few are left, the remaining places hold
- * the index E and the weight 0. An expert with a NaN is never chosen, and a row with a NaN logit has NaN weights.
+ * Without bias and TTB_GROUP_TOP2_SUM the order is that of the logits, which is that of their exact scores: two scores that only rounding to 64 bits makes equal (a
+ * sigmoid above about 37) do not tie. With either, order and ties are those of 64-bit choice values and sums, in which such scores do. An expert with logit or
+ * bias -inf is never chosen; where too few are left, the remaining places hold the index E and the weight 0. An expert with a NaN is never chosen, and a row with a
+ * NaN logit has NaN weights.
  * E up to 1024, k up to 32, up to 32 groups. */
 int32_t ttb_route_to_experts(const void *logits_dev, int32_t logits_dtype, const void *bias_dev, void *weights_dev, void *experts_dev, int64_t outer, int64_t H,
                              int64_t E, int32_t k, int32_t score, int32_t groups, int32_t top_groups, int32_t group_score, int32_t renormalize, float scale,

@@ -145,3 +145,19 @@ def test_linear_columns_that_only_pad_are_zero(dev, rows, k, n, dtype, act):
         full = ttnn.to_torch(y.reshape(ttnn.Shape(list(y.shape.padded))))
         assert full.shape[-1] > n and (full[:, n:] == 0).all()
         assert torch.isfinite(full[[0, 2, 21, 30]]).all()
+
+
+# ---- the router's order where scores saturate ------------------------------------------------------------------------------
+@pytest.mark.parametrize("score,logits", [("sigmoid", [60.0, 62.0, 61.0, 62.0, 0.0, 59.0, 60.0, 63.0]), ("softmax", [0.0, -900.0, -800.0, -900.0, -1000.0, -800.0, -850.0, -950.0])])
+def test_route_order_of_saturated_scores(dev, score, logits):
+    """By the logits without bias and group sums, though the 64-bit scores of most of these are equal; else by the 64-bit scores, ties to the lowest index."""
+    x = torch.tensor([logits], dtype=torch.double)
+    s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1)
+    by_logit, by_score = (sorted(range(8), key=lambda i: (-v[0, i].item(), i)) for v in (x, s))
+    assert by_logit != by_score
+    t = put(x.float(), dev)
+
+    def ids(**kw):
+        return ttnn.to_torch(ttnn.route_to_experts(t, 8, score=score, **kw)[1])[0].tolist()
+    assert ids() == by_logit == ids(groups=2, top_groups=2)
+    assert ids(bias=put(torch.zeros(8), dev)) == by_score == ids(groups=2, top_groups=2, group_score="top2_sum")

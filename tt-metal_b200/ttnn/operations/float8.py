@@ -53,7 +53,8 @@ def route_to_experts(logits, k: int, *, score: str = "softmax", bias=None, group
     Scores are the softmax or sigmoid of the logits. Experts are chosen by score + bias (`bias`: float32, one value an expert, for balance), ties to the
     lowest index; with groups > 1 only among the top_groups groups of E / groups neighbouring experts whose best expert (group_score "max") or two best
     together ("top2_sum") count most. Weights are the chosen experts' scores (without bias) times `scale`, divided by their sum under `renormalize`.
-    The order is that of 64-bit values. An expert whose logit is -inf is never chosen; where a row has too few left, the remaining places hold the index E
+    Without bias and "top2_sum" the order is that of the logits, which is that of exact scores; with either it is that of 64-bit scores and sums, in which scores that
+    only differ behind 64 bits (sigmoids of logits above about 37) are ties. An expert whose logit is -inf is never chosen; where a row has too few left, the remaining places hold the index E
     and the weight 0 (ttnn.experts_mlp_float8 skips them: a row of -inf gets no expert). The experts of a row with a NaN, or an infinity
     under softmax, have NaN weights; a NaN's own is never chosen."""
     weights, experts = _ttnn.route_to_experts(_unwrap(logits), k, score=score, bias=_unwrap(bias) if bias is not None else None, groups=groups,
