@@ -273,15 +273,14 @@ extern "C" int32_t ttb_quantize_float8(const void *src, int32_t src_dtype, int32
         return fail(TTB_E_INVALID, "ttb_quantize_float8: misaligned pointer");
     const ttb::Source s = ttb::make_source(src, src_dtype, src_row_major != 0, H, W);
     const bool vector_out = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && W % 8 == 0;
-    if (outer * H > INT32_MAX || outer * H * ttb::f8_blocks(W) > INT32_MAX) return fail(TTB_E_UNSUPPORTED, "ttb_quantize_float8: too many blocks");
+    const int64_t row_blocks = block_rows == 1 ? outer * H : outer * ttb::f8_blocks(H), blocks = row_blocks * ttb::f8_blocks(W);
+    if (outer * H > INT32_MAX || blocks > INT32_MAX) return fail(TTB_E_UNSUPPORTED, "ttb_quantize_float8: too many blocks");
     if (block_rows == 1) {
-        const int64_t want = (outer * H * ttb::f8_blocks(W) + 15) / 16;
+        const int64_t want = (blocks + 15) / 16;
         const unsigned grid = (unsigned)(want < 148 * 6 ? want : 148 * 6);
         auto kernel = src_dtype == TTB_FLOAT32 ? ttb::quantize_rows_kernel<float> : ttb::quantize_rows_kernel<uint16_t>;
         kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(s, (uint8_t *)codes, (float *)scales, outer * H, H, W, vector_out);
     } else {
-        const int64_t blocks = outer * ttb::f8_blocks(H) * ttb::f8_blocks(W);
-        if (blocks > INT32_MAX) return fail(TTB_E_UNSUPPORTED, "ttb_quantize_float8: too many blocks");
         auto kernel = src_dtype == TTB_FLOAT32 ? ttb::quantize_blocks_kernel<float> : ttb::quantize_blocks_kernel<uint16_t>;
         kernel<<<(unsigned)blocks, 512, 0, (cudaStream_t)stream>>>(s, (uint8_t *)codes, (float *)scales, H, W, vector_out);
     }
