@@ -161,3 +161,30 @@ def test_route_order_of_saturated_scores(dev, score, logits):
         return ttnn.to_torch(ttnn.route_to_experts(t, 8, score=score, **kw)[1])[0].tolist()
     assert ids() == by_logit == ids(groups=2, top_groups=2)
     assert ids(bias=put(torch.zeros(8), dev)) == by_score == ids(groups=2, top_groups=2, group_score="top2_sum")
+
+
+# ---- unusual routes, with inputs that are the same in every run ------------------------------------------------------------
+@pytest.mark.parametrize("seed,kind", list(enumerate(["none", "one", "all_to_last", "twice", "outside", "negative_weights"])))
+@pytest.mark.parametrize("rows", [5, 90, 400])
+def test_experts_with_unusual_routes_of_fixed_seeds(dev, rows, seed, kind):
+    g = gen(100 * rows + seed)
+    e, k, hidden, ffn = 6, 3, 256, 384
+    x, ws = ref.rows_of(g, rows, hidden), [ref.weight(g, *s, (e,)) for s in ((ffn, hidden), (ffn, hidden), (hidden, ffn))]
+    best, ids = (torch.randn(rows, e, generator=g) + torch.randn(e, generator=g)).topk(k, -1)
+    ids, p = ids.int(), best.softmax(-1)
+    if kind == "none":
+        ids[:] = e
+    elif kind == "one":
+        ids[:], ids[rows // 2, 1] = e, 2
+    elif kind == "all_to_last":
+        ids[:], ids[:, 0] = e, e - 1
+    elif kind == "twice":
+        ids[:, 1] = ids[:, 0]
+    elif kind == "outside":
+        ids[::3], ids[1::3, 0], ids[2] = -1, 1 << 30, -(1 << 31)
+    else:
+        p = p - 0.5
+    y = ttnn.to_torch(ttnn.experts_mlp_float8(put(x, dev), put(ids, dev), put(p, dev), *[pair(w, dev) for w in ws]))
+    want, tol = ref.experts(x.cuda(), ids.cuda(), p.cuda(), *[(a.cuda(), b.cuda()) for a, b in ws])
+    ref.assert_within(y, want, tol, kind)
+    assert (y[((ids < 0) | (ids >= e)).all(1)] == 0).all()
