@@ -1,5 +1,6 @@
 """float8 operators where their contract is easy to miss: codes of the experts' inner quantisation, rows that are not finite under activations and in the
 padding of tiled results, saturated router scores."""
+import ctypes
 import math
 
 import pytest
@@ -8,6 +9,7 @@ import torch
 import cabi
 import float8_ref as ref
 import ttnn
+from test_matmul_gpu import make_case
 from test_float8_gpu import dev, no_wait_ran_out, pair, put, same_bits  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
@@ -188,3 +190,78 @@ def test_experts_with_unusual_routes_of_fixed_seeds(dev, rows, seed, kind):
     want, tol = ref.experts(x.cuda(), ids.cuda(), p.cuda(), *[(a.cuda(), b.cuda()) for a, b in ws])
     ref.assert_within(y, want, tol, kind)
     assert (y[((ids < 0) | (ids >= e)).all(1)] == 0).all()
+
+
+# ---- behind a wait that ran out --------------------------------------------------------------------------------------------
+def _peer_matmul_that_waits_in_vain(lib, orc, workspace):
+    """A block-float matmul whose activations other GPUs never deliver, on the workspace; it gives up at the limit of its launch."""
+    x, w, _ = make_case(lib, orc, 18, 32, 4096, 512, cabi.BFLOAT8_B)
+    a, out = lib.tilize(x.cuda(), 1, 32, 4096), torch.zeros(32 * 512, dtype=torch.bfloat16, device="cuda")
+    counters = torch.zeros(64, dtype=torch.int32, device="cuda")
+    counters[32] = 1
+    torch.cuda.synchronize()
+    wait = cabi.peer_wait(counters.data_ptr(), counters.data_ptr() + 128)
+
+    def call():
+        lib.check(lib.cdll.ttb_matmul_peer(a.data_ptr(), cabi.BFLOAT16, w.data_ptr(), cabi.BFLOAT8_B, None, out.data_ptr(), cabi.BFLOAT16, 1, 32, 4096, 512, 0,
+                                           cabi.MM_WORKSPACE_ZEROED, workspace.data_ptr(), workspace.numel(), None, ctypes.byref(wait), None))
+    call.keep = a, out, counters, w
+    return call
+
+
+@pytest.mark.parametrize("rows", [1, 40, 200])
+def test_linear_behind_a_kernel_that_waits_for_peers(ttb, orc, rows):
+    """The kernel in front waits 1.3 s and gives up; the float8 kernels, which start while it waits, do not count that time under their limit of about a second."""
+    c = ref.lib()
+    g = gen(7)
+    x, w = ref.rows_of(g, rows, 2048).cuda(), [t.cuda() for t in ref.weight(g, 1000, 2048)]
+    need = c.ttb_linear_float8_workspace_bytes(rows, 2048, 1000)
+    spaces = [torch.zeros(max(need, 65536 + (48 << 20)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    out = torch.zeros(rows, 1000, dtype=torch.float32, device="cuda")
+
+    def linear(space, flags):
+        assert c.ttb_linear_float8(x.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), None, out.data_ptr(), 1, rows, 2048, 1000, 0, 3 | flags, space.data_ptr(), need, None) == 0
+    linear(spaces[0], cabi.MM_WORKSPACE_ZEROED)
+    assert ttb.check_status(None) == 0
+    want, tol = ref.linear(x, *w, None, None, torch.float32)
+    ref.assert_within(out, want, tol)
+    out.zero_()
+    wait = _peer_matmul_that_waits_in_vain(ttb, orc, spaces[1])
+    ttb.check(ttb.set_wait_limit_cycles(2_600_000_000))
+    try:
+        wait()
+    finally:
+        ttb.check(ttb.set_wait_limit_cycles(0))
+    linear(spaces[0], cabi.MM_WORKSPACE_ZEROED | cabi.MM_WEIGHTS_RESIDENT)
+    assert ttb.check_status(None) == -5
+    assert int(ttb.cdll.ttb_last_error().decode().split("wait site ")[1].rstrip(")")) < 40   # (the kernel in front)
+    assert ttb.check_status(None) == 0
+    ref.assert_within(out, want, tol)
+    # the workspace that the matmul gave up on: trusted again once its head is clear, or by a call that clears the counters itself
+    for flags in (0, cabi.MM_WORKSPACE_ZEROED):
+        out.zero_()
+        if flags:
+            spaces[1][: 65536 + (16 << 20)].zero_()
+        linear(spaces[1], flags)
+        ref.assert_within(out, want, tol)
+    assert ttb.check_status(None) == 0
+
+
+def test_surface_linear_after_a_timeout(ttb, orc, dev):
+    """The host layer raises once and clears its scratch; the next linear is right."""
+    g = gen(8)
+    x, w = ref.rows_of(g, 40, 8192), ref.weight(g, 1000, 8192)
+    xt, wt = put(x, dev), pair(w, dev)
+    want, tol = ref.linear(x.cuda(), w[0].cuda(), w[1].cuda(), None, None, torch.bfloat16)
+    ref.assert_within(ttnn.to_torch(ttnn.linear_float8(xt, wt)), want, tol)
+    space = torch.zeros(65536 + (48 << 20), dtype=torch.uint8, device="cuda")
+    wait = _peer_matmul_that_waits_in_vain(ttb, orc, space)
+    ttb.check(ttb.set_wait_limit_cycles(2_000_000))
+    try:
+        wait()
+    finally:
+        ttb.check(ttb.set_wait_limit_cycles(0))
+    with pytest.raises(RuntimeError, match="ran out"):
+        ttnn.synchronize_device(dev)
+    for _ in range(2):
+        ref.assert_within(ttnn.to_torch(ttnn.linear_float8(xt, wt)), want, tol)
