@@ -23,7 +23,7 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
+constexpr int kMaxExperts = kF8MaxExperts, kMaxTopK = 32, kMaxGroups = 32;
 constexpr int kRouteWarps = 4;
 
 struct RouteArgs {
@@ -355,9 +355,6 @@ int32_t launch_route(const RouteArgs &p, cudaStream_t stream) {
     return TTB_OK;
 }
 
-int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-bool misaligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
-
 // Scratch of the experts' MLP.
 struct Scratch {
     int64_t assignments;
@@ -368,35 +365,25 @@ struct Scratch {
     float *partials;                         // of either matmul, one after the other
     int64_t bytes;
 };
-F8Activation place(uint8_t *base, int64_t &at, int64_t rows, int64_t cols) {
-    F8Activation a;
-    a.rows_padded = f8_rows_padded(rows);
-    a.scale_pitch = f8_scale_pitch(cols);
-    a.codes = base + at;
-    at = up(at + a.rows_padded * f8_blocks(cols) * kF8Block, 1024);
-    a.scales = reinterpret_cast<float *>(base + at);
-    at = up(at + a.rows_padded * a.scale_pitch * 4, 1024);
-    return a;
-}
 Scratch lay_out(uint8_t *base, int64_t rows, int64_t experts, int64_t k, int64_t hidden, int64_t ffn) {
     Scratch s;
     s.assignments = rows * k;
     int64_t at = 0;
     s.offsets = reinterpret_cast<int32_t *>(base + at);
-    at = up(at + 4 * (experts + 1), 1024);
+    at = f8_up(at + 4 * (experts + 1), 1024);
     s.pos = reinterpret_cast<int32_t *>(base + at);
-    at = up(at + 4 * s.assignments, 1024);
+    at = f8_up(at + 4 * s.assignments, 1024);
     s.row_of = reinterpret_cast<int32_t *>(base + at);
-    at = up(at + 4 * s.assignments, 1024);
-    s.x = f8_quantises_itself(s.assignments, experts) ? F8Activation{} : place(base, at, s.assignments, hidden);
-    s.h = place(base, at, s.assignments, ffn);
+    at = f8_up(at + 4 * s.assignments, 1024);
+    s.x = f8_quantises_itself(s.assignments, experts) ? F8Activation{} : f8_place(base, at, s.assignments, hidden);
+    s.h = f8_place(base, at, s.assignments, ffn);
     s.y = reinterpret_cast<float *>(base + at);
-    at = up(at + s.assignments * hidden * 4, 1024);
+    at = f8_up(at + s.assignments * hidden * 4, 1024);
     s.gated_tickets = reinterpret_cast<int32_t *>(base + at);
     s.down_tickets = reinterpret_cast<int32_t *>(base + at + kF8TicketBytes);
     at += 2 * kF8TicketBytes;
     s.partials = reinterpret_cast<float *>(base + at);
-    at += f8_partial_bytes(s.assignments, true);
+    at += f8_partial_bytes(s.assignments);
     s.bytes = at;
     return s;
 }
@@ -425,7 +412,7 @@ int32_t ttb_route_to_experts(const void *logits, int32_t logits_dtype, const voi
     if (top_groups < 1 || top_groups > groups) return fail(TTB_E_INVALID, "%s: top_groups must be between 1 and the number of groups", who);
     if (k > E / groups * top_groups) return fail(TTB_E_INVALID, "%s: %d groups of %lld experts have no %d to choose", who, top_groups, (long long)(E / groups), k);
     if (group_score != TTB_GROUP_MAX && group_score != TTB_GROUP_TOP2_SUM) return fail(TTB_E_INVALID, "%s: unknown group score %d", who, group_score);
-    if (ttb::misaligned(logits, logits_dtype == TTB_FLOAT32 ? 4 : 2) || (bias && ttb::misaligned(bias, 4)) || ttb::misaligned(weights, 4) || ttb::misaligned(experts, 4))
+    if (ttb::f8_misaligned(logits, logits_dtype == TTB_FLOAT32 ? 4 : 2) || (bias && ttb::f8_misaligned(bias, 4)) || ttb::f8_misaligned(weights, 4) || ttb::f8_misaligned(experts, 4))
         return fail(TTB_E_INVALID, "%s: misaligned tensor", who);
     ttb::RouteArgs p;
     p.logits = logits; p.bias = (const float *)bias; p.weights = (float *)weights; p.experts = (int32_t *)experts;
@@ -460,9 +447,9 @@ int32_t ttb_experts_mlp_float8(const void *x, const void *ids, const void *weigh
         return fail(TTB_E_INVALID, "%s: between 1 and 2^24 rows times k, hidden and ffn sizes of at most 2^24, 1 to %d experts and k of 1 to %d", who, ttb::kMaxExperts, ttb::kMaxTopK);
     if (hidden % 16 || ffn % 16) return fail(TTB_E_INVALID, "%s: the hidden and ffn sizes must be multiples of 16 (got %lld, %lld)", who, (long long)hidden, (long long)ffn);
     for (const void *p : {x, gate_codes, up_codes, down_codes, (const void *)out})
-        if (ttb::misaligned(p, 16)) return fail(TTB_E_INVALID, "%s: activations, codes and the result must be 16-byte aligned", who);
+        if (ttb::f8_misaligned(p, 16)) return fail(TTB_E_INVALID, "%s: activations, codes and the result must be 16-byte aligned", who);
     for (const void *p : {ids, weights, gate_scales, up_scales, down_scales})
-        if (ttb::misaligned(p, 4)) return fail(TTB_E_INVALID, "%s: misaligned tensor", who);
+        if (ttb::f8_misaligned(p, 4)) return fail(TTB_E_INVALID, "%s: misaligned tensor", who);
     if (!ttb::workspace_serves(workspace, workspace_bytes, need)) return fail(TTB_E_WORKSPACE, "%s: needs %lld bytes of 256-byte aligned workspace", who, (long long)need);
     const cudaStream_t s = (cudaStream_t)stream;
     const bool x_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;

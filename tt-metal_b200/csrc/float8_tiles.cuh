@@ -14,9 +14,9 @@ namespace f8 {
 using namespace ptx;
 
 constexpr int kMaxStages = 12;
-constexpr int kEpiWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kIssuers = 2, kThreads = 32 * 12;   // (the last warp completes the warpgroup that hands registers on)
+constexpr int kEpiWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kIssuers = 2;
+constexpr int kQuantRows = 8;               // rows of a tile whose kernel quantises them itself
 constexpr int kSmemLimit = 232448 - 3072;   // the rest: static shared memory
-constexpr int kMaxExperts = 1024;
 
 struct alignas(64) Args {
     CUtensorMap wmap[2];
@@ -74,7 +74,6 @@ __device__ __forceinline__ void fma_pair(float &a0, float &a1, uint32_t r0, uint
         : "+f"(a0), "+f"(a1)
         : "r"(r0), "r"(r1), "l"(f));
 }
-__device__ __forceinline__ uint64_t twice(float f) { return ((uint64_t)__float_as_uint(f) << 32) | __float_as_uint(f); }
 
 // Adds an accumulator's NC columns, times f0 (gated: the second half times f1), to the sums, 32 at a time, the next 32 on their way meanwhile. column(j): that of
 // sum j; free() is called as soon as the accumulator may be written again.
@@ -97,7 +96,8 @@ __device__ __forceinline__ void add_accumulator(uint32_t t0, float f0, float f1,
     for (int q = 0; q < NC; q += 32) {
         if (q + 32 < NC) load(q + 32, r[(q / 32 + 1) & 1]);
         else free();
-        const uint64_t f = twice(GATED && q >= NC / 2 ? f1 : f0);
+        const float factor = GATED && q >= NC / 2 ? f1 : f0;
+        const uint64_t f = f8_two(factor, factor);
 #pragma unroll
         for (int j = 0; j < 32; j += 2) fma_pair(acc[q + j], acc[q + j + 1], r[(q / 32) & 1][j], r[(q / 32) & 1][j + 1], f);
         if (q + 32 < NC) tmem_ld_wait();

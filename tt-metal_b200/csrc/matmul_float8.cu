@@ -328,16 +328,17 @@ int32_t launch(const Args &p, int grid, int smem, int dev, cudaStream_t stream) 
 }  // namespace
 
 static int partial_rows(int64_t rows) { return rows >= BM - 31 ? BM : (int)(f8_rows_padded(rows) + 31) / 32 * 32; }
-int64_t f8_partial_bytes(int64_t rows, bool gated) { return 2 * (int64_t)stream_blocks() * partial_rows(rows) * 128 * 2 * 4; }
+int64_t f8_partial_bytes(int64_t rows) { return 2 * (int64_t)stream_blocks() * partial_rows(rows) * 128 * 2 * 4; }
 
-// Rows of a tile, by all rows or by what an expert has on average.
-static int rows_per_tile(int64_t rows, int64_t experts) {
-    const int64_t hit = rows < experts ? rows : experts, mean = experts ? (rows + hit - 1) / hit : rows;
-    return mean <= (experts ? 24 : 32) ? 32 : mean <= (experts ? 56 : 64) ? 64 : BM;
-}
+// All rows, or what an expert has on average.
 static int64_t mean_rows(int64_t rows, int64_t experts) {
     const int64_t hit = rows < experts ? rows : experts;
     return experts ? (rows + hit - 1) / hit : rows;
+}
+// Rows of a tile.
+static int rows_per_tile(int64_t rows, int64_t experts) {
+    const int64_t mean = mean_rows(rows, experts);
+    return mean <= (experts ? 24 : 32) ? 32 : mean <= (experts ? 56 : 64) ? 64 : BM;
 }
 bool f8_quantises_itself(int64_t rows, int64_t experts) { return mean_rows(rows, experts) <= (experts ? 4 : 8); }
 
@@ -359,7 +360,7 @@ static int weight_blocks(const F8Matmul &m, int R, int64_t sms) {
 int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     Args p;
     const int64_t experts = m.experts ? m.experts : 1;
-    if (m.experts > kMaxExperts) return fail(TTB_E_UNSUPPORTED, "ttb_experts_mlp_float8: at most %d experts", kMaxExperts);
+    if (m.experts > kF8MaxExperts) return fail(TTB_E_UNSUPPORTED, "ttb_experts_mlp_float8: at most %d experts", kF8MaxExperts);
     if (int32_t rc = make_map(m.w[0].codes, experts, m.N, m.K, p.wmap[0])) return rc;
     p.wmap[1] = p.wmap[0];
     if (m.gated)
@@ -384,7 +385,7 @@ int32_t launch_matmul_float8(const F8Matmul &m, cudaStream_t stream) {
     p.partials = m.partials;
     p.partial_rows = partial_rows(m.rows);
     p.ct = m.gated ? p.Nb : (p.Nb + W - 1) / W;
-    p.tile_rows = m.x.ptr ? 8 : R;
+    p.tile_rows = m.x.ptr ? kQuantRows : R;
     p.a_rows = (int)(f8_rows_padded(m.rows) < p.tile_rows ? f8_rows_padded(m.rows) : p.tile_rows);
     p.stage_bytes = p.a_rows * kF8Block + W * kF8BlockBytes;
     const int extra = (R < BM ? p.tile_rows * 128 * W * 4 : m.gated ? 2 * BM * 4 : 0) + (m.experts ? 4 * (2 * m.experts + 1) : 0) + 1024;
@@ -420,30 +421,14 @@ namespace {
 // they leave alone.
 constexpr int64_t kWorkspaceHead = 65536 + (int64_t(16) << 20);
 constexpr int64_t kMaxExtent = int64_t(1) << 24;   // rows, K and N: tile coordinates and row indexes stay far inside 32 bits
-
-int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-
-bool misaligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
-
-// Scratch of quantised rows; advances `at`.
-ttb::F8Activation place(uint8_t *base, int64_t &at, int64_t rows, int64_t cols) {
-    ttb::F8Activation a;
-    a.rows_padded = ttb::f8_rows_padded(rows);
-    a.scale_pitch = ttb::f8_scale_pitch(cols);
-    a.codes = base + at;
-    at = up(at + a.rows_padded * ttb::f8_blocks(cols) * ttb::kF8Block, 1024);
-    a.scales = reinterpret_cast<float *>(base + at);
-    at = up(at + a.rows_padded * a.scale_pitch * 4, 1024);
-    return a;
-}
 }  // namespace
 
 extern "C" {
 
 int64_t ttb_linear_float8_workspace_bytes(int64_t rows, int64_t K, int64_t N) {
     if (rows <= 0 || K <= 0 || N <= 0 || rows > kMaxExtent || K > kMaxExtent || N > kMaxExtent) return -1;
-    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows, false);
-    if (!ttb::f8_quantises_itself(rows, 0)) place(nullptr, at, rows, K);
+    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows);
+    if (!ttb::f8_quantises_itself(rows, 0)) ttb::f8_place(nullptr, at, rows, K);
     return at;
 }
 
@@ -458,14 +443,15 @@ int32_t ttb_linear_float8(const void *a, const void *w_codes, const void *w_scal
     if (K % 16) return fail(TTB_E_INVALID, "ttb_linear_float8: K must be a multiple of 16 (got %lld)", (long long)K);
     const bool a_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;
     if ((!a_rm || !out_rm) && rows % 32) return fail(TTB_E_INVALID, "ttb_linear_float8: tiled tensors have a multiple of 32 rows (got %lld)", (long long)rows);
-    if (misaligned(a, 16) || misaligned(w_codes, 16) || misaligned(w_scales, 4) || misaligned(out, out_dtype == TTB_FLOAT32 ? 4 : 2) || (bias && misaligned(bias, 2)))
+    if (ttb::f8_misaligned(a, 16) || ttb::f8_misaligned(w_codes, 16) || ttb::f8_misaligned(w_scales, 4) || ttb::f8_misaligned(out, out_dtype == TTB_FLOAT32 ? 4 : 2) ||
+        (bias && ttb::f8_misaligned(bias, 2)))
         return fail(TTB_E_INVALID, "ttb_linear_float8: activations and codes must be 16-byte aligned, the other tensors as their elements");
     if (!ttb::workspace_serves(workspace, workspace_bytes, need)) return fail(TTB_E_WORKSPACE, "ttb_linear_float8: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     ttb::F8Matmul m = {};
     m.tickets = static_cast<int32_t *>(workspace);
     m.partials = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kWorkspaceHead);
-    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows, false);
-    m.a = place(static_cast<uint8_t *>(workspace), at, rows, K);
+    int64_t at = kWorkspaceHead + ttb::f8_partial_bytes(rows);
+    m.a = ttb::f8_place(static_cast<uint8_t *>(workspace), at, rows, K);
     m.w[0] = {w_codes, static_cast<const float *>(w_scales)};
     m.rows = rows; m.K = K; m.N = N;
     m.act = activation;

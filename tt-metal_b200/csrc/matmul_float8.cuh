@@ -12,6 +12,20 @@ struct F8Activation {
     int64_t scale_pitch;
 };
 
+inline int64_t f8_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+inline bool f8_misaligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+// Scratch of quantised rows; advances `at`.
+inline F8Activation f8_place(uint8_t *base, int64_t &at, int64_t rows, int64_t cols) {
+    F8Activation a;
+    a.rows_padded = f8_rows_padded(rows);
+    a.scale_pitch = f8_scale_pitch(cols);
+    a.codes = base + at;
+    at = f8_up(at + a.rows_padded * f8_blocks(cols) * kF8Block, 1024);
+    a.scales = reinterpret_cast<float *>(base + at);
+    at = f8_up(at + a.rows_padded * a.scale_pitch * 4, 1024);
+    return a;
+}
+
 // bfloat16 rows that a kernel quantises itself: row r is row_of[r] of `ptr` (null: r itself).
 struct F8Rows {
     const uint16_t *ptr;
@@ -48,8 +62,9 @@ struct F8Matmul {
     int32_t *tickets;   // kF8TicketBytes, zero when the kernel starts and when it ends
     float *partials;    // f8_partial_bytes, no particular contents
 };
+constexpr int kF8MaxExperts = 1024;
 constexpr int64_t kF8TicketBytes = 8192;
-int64_t f8_partial_bytes(int64_t rows, bool gated);
+int64_t f8_partial_bytes(int64_t rows);
 int32_t launch_matmul_float8(const F8Matmul &p, cudaStream_t stream);
 // Whether the kernel for these row counts quantises the activations itself.
 bool f8_quantises_itself(int64_t rows, int64_t experts);

@@ -25,7 +25,6 @@ constexpr int few_threads(bool quant) { return 32 * (quant ? kQuantWarp0 + kQuan
 // A quantising warp takes the units of every fourth stage, of at most kQuantRows rows: 16 lanes have 128 values of a row, the loads run one unit of the warp's
 // ahead. (Stages, not units, are dealt out: a wait for a phase's parity means something only to a warp that has waited for the stage's phase before it. Dealt by
 // units, with five stages, a warp could overtake another's MMAs by a whole round of the ring, and did: the block left with copies under way.)
-constexpr int kQuantRows = 8;
 __device__ __forceinline__ void quantise(const Args &p, const Ring &ring, uint8_t *smem, uint32_t ready0, float *scales, Walk walk, const int *off, const int *cum, int which) {
     grid_dep_wait();
     const int lane = threadIdx.x & 31, sub = lane & 15, r0 = lane >> 4;
@@ -103,7 +102,7 @@ __device__ __forceinline__ void quantise(const Args &p, const Ring &ring, uint8_
 template <int ACT, int W, int R, bool GATED, bool QUANT>
 __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kernel(const __grid_constant__ Args p) {
     static_assert(!GATED || W == 2, "a gated tile takes a block of either weight");
-    static_assert(!QUANT || R == 32, "tiles of kQuantRows rows");
+    static_assert(!QUANT || (R == 32 && kQuantRows == 8), "half a warp has every other row of a tile, four at most");
     constexpr int NR = R * W / 2;             // rows of an epilogue thread: all of them of weight block `half`, or half of the rows of the one block
     constexpr int NX = NR > 32 ? 2 : 1;       // registers that hold a scale of each
     constexpr bool ADD = R <= 32;
