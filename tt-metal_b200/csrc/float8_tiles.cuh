@@ -213,6 +213,7 @@ struct Walk {
 struct Ring {
     uint32_t sbase, full0, done0, acc0;
     volatile int *abort_flag;
+    volatile int *progress;   // the unit that is fetched, at most the ring's stages ahead of the adding warps
     __device__ uint32_t full(int s) const { return full0 + 8u * s; }
     __device__ uint32_t done(int s) const { return done0 + 8u * s; }
     __device__ uint32_t acc_empty(int b) const { return acc0 + 8u * b; }
@@ -252,7 +253,10 @@ __device__ __forceinline__ void fetch(const Args &p, const Ring &ring, Walk walk
         for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
             if (n >= ahead) {
                 if (!__all_sync(0xffffffffu, mbar_wait(ring.done(s), ph ^ 1, ring.abort_flag, p.status, 51, wait_clocks(p)))) return;
-                if (leader) fetch_weights(s, T, kb);
+                if (leader) {
+                    fetch_weights(s, T, kb);
+                    *ring.progress = n;
+                }
             }
             if (!QUANT && leader) bulk_g2s_plain(ring.stage(p, s), p.a.codes + ((int64_t)kb * p.a.rows_padded + T.base) * kF8Block, a_bytes(T), ring.full(s));
             if (++s == p.stages) { s = 0; ph ^= 1; }
@@ -378,11 +382,6 @@ __device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, 
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = activate<ACT>(v[j]);
-    if (n + 16 > p.N) {   // (columns that only pad a tile: a NaN or an infinity of the row times the zeros behind the weight's last row is a NaN)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (n + j >= p.N) v[j] = 0.0f;
-    }
     store16(p, row, n, v);
 }
 
@@ -390,6 +389,11 @@ __device__ __forceinline__ void finish16(const Args &p, int64_t row, int64_t n, 
 // runs cold once a tile (a 350 x 4544 x 4672 launch with gelu: 39 us against 21 without finishing its tiles).
 template <int ACT, int NC>
 __device__ __forceinline__ void finish_row(const Args &p, int64_t row, int64_t n0, float (&acc)[NC]) {
+    if (!p.out_row_major && n0 + NC > p.N) {   // columns that only pad a tile: a NaN or an infinity of the row times the zeros behind the weight's last row is a NaN
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            if (n0 + j >= p.N) acc[j] = 0.0f;
+    }
     if constexpr (ACT == TTB_ACT_NONE) {
 #pragma unroll
         for (int q = 0; q < NC; q += 16) finish16<ACT>(p, row, n0 + q, acc + q);
@@ -448,7 +452,7 @@ __device__ __forceinline__ void finish4(const Args &p, int64_t row, int64_t n, f
             if (n + j < p.N) v[j] += __uint_as_float((uint32_t)b[j] << 16);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = n + j < p.N ? activate<ACT>(v[j]) : 0.0f;   // (as in finish16)
+    for (int j = 0; j < 4; ++j) v[j] = n + j < p.N ? activate<ACT>(v[j]) : 0.0f;   // (as in finish_row)
     const int64_t off = p.out_row_major ? row * p.N + n : tiled_offset(row, n, width >> 5);
     const bool f32 = p.out_dtype == TTB_FLOAT32;
     if (p.out_aligned >= 16 && n + 4 <= width) {
@@ -540,21 +544,22 @@ __device__ __forceinline__ void add_parts(const Args &p, F part_of, int c0, int 
     }
 }
 
-// mbar_wait for what lies any number of units ahead: the limit is for the time without progress, the number of the unit that the adding warps are at. (A wait with
-// one limit for all of it would run out in a sound launch that is longer than the limit.)
-__device__ __forceinline__ bool wait_while_units_pass(uint32_t bar, uint32_t parity, volatile int *progress, volatile int *abort_flag, int *status, int code, long long limit) {
+// mbar_wait for what lies any number of units ahead: the limit is for the time in which no unit is fetched. (A wait with one limit for all of it would run out in a
+// sound launch that is longer than the limit. The fetching warp has the time to say where it is: a store a unit in the adding warps cost 4 % of 2048 rows on experts,
+// one in the issuing warps 1 % of 2048 x 8192 x 28672.)
+__device__ __forceinline__ bool wait_while_units_pass(const Ring &ring, uint32_t bar, uint32_t parity, int *status, int code, long long limit) {
     if (mbar_try_wait(bar, parity)) return true;
-    int at = *progress;
+    int at = *ring.progress;
     long long t0 = clock64();
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_try_wait_suspend(bar, parity, 4000u)) return true;
         if ((spin & 7u) == 0u) {
-            if (*abort_flag) return false;
-            if (*progress != at) {
-                at = *progress;
+            if (*ring.abort_flag) return false;
+            if (*ring.progress != at) {
+                at = *ring.progress;
                 t0 = clock64();
             } else if (clock64() - t0 > limit) {
-                *abort_flag = 1;
+                *ring.abort_flag = 1;
                 atomicCAS(status, 0, code);
                 return false;
             }
@@ -566,13 +571,13 @@ __device__ __forceinline__ bool wait_while_units_pass(uint32_t bar, uint32_t par
 // `handed` says that its part is written. Where all parts are there with it, it finishes the tile itself if it has few rows (ADD), else the adding warps do it after
 // their last segment (`pending`: the tile, or -1; then `told`): one warp alone took 126 x 18272 x 6376 from 47 to 83 us.
 template <int ACT, int W, bool GATED, bool ADD>
-__device__ __forceinline__ void hand_over(const Args &p, uint32_t handed, uint32_t told, volatile int *pending, volatile int *progress, volatile int *abort_flag, Walk walk, const int *off, const int *cum) {
+__device__ __forceinline__ void hand_over(const Args &p, uint32_t handed, uint32_t told, volatile int *pending, const Ring &ring, Walk walk, const int *off, const int *cum) {
     grid_dep_wait();
     const int lane = threadIdx.x & 31;
     Segment seg;
     while (walk.next(seg)) {
         if (seg.kb1 - seg.kb0 == p.Kb || walk.u >= walk.u_end) continue;
-        if (!__all_sync(0xffffffffu, wait_while_units_pass(handed, 0, progress, abort_flag, p.status, 56, wait_clocks(p)))) return;
+        if (!__all_sync(0xffffffffu, wait_while_units_pass(ring, handed, 0, p.status, 56, wait_clocks(p)))) return;
         const Sharing sh(walk, seg);
         int last = 0;
         if (lane == 0) last = take_ticket(p.tickets + sh.q) == sh.c1 - sh.c0;

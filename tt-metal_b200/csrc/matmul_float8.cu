@@ -71,7 +71,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
     auto pair = [&](int quad) { return bar0 + 8u * (2 * kMaxStages + 4 + quad); };
     const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + 8), handed_bar = all_bar + 8, told_bar = handed_bar + 8;
     volatile int *abort_flag = &abort_word;
-    const Ring ring = {sbase, bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag};
+    const Ring ring = {sbase, bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag, &progress};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -114,7 +114,7 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
                     mma_e4m3_ss(tmem_base + (uint32_t)(buf * 128 * W), a + 2 * k, b + 2 * k, instr_desc_e4m3(BM, 128 * W), k > 0);
             });
         } else {
-            hand_over<ACT, W, GATED, false>(p, handed_bar, told_bar, &pending, &progress, abort_flag, walk, off, cum);
+            hand_over<ACT, W, GATED, false>(p, handed_bar, told_bar, &pending, ring, walk, off, cum);
         }
     } else {
         if (W == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
@@ -170,7 +170,6 @@ __global__ void __maxnreg__(kRegs) matmul_float8_kernel(const __grid_constant__ 
             for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
             for (int kb = now.kb0; kb < now.kb1; ++kb, ++n) {
                 const int buf = n % NB;
-                if (threadIdx.x == 0) progress = n;
                 const float x = (kb & 2) ? ((kb & 1) ? c.xa.w : c.xa.z) : ((kb & 1) ? c.xa.y : c.xa.x);
                 const float f0 = x * __shfl_sync(0xffffffffu, c.w0, kb & 31), f1 = GATED ? x * __shfl_sync(0xffffffffu, c.w1, kb & 31) : f0;
                 if ((kb & 3) == 3) {

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     int *cum = off + p.experts + 1;
     const uint32_t bar0 = smem_u32(bars);
     volatile int *abort_flag = &abort_word;
-    const Ring ring = {smem_u32(smem), bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag};
+    const Ring ring = {smem_u32(smem), bar0, bar0 + 8u * kMaxStages, bar0 + 8u * (2 * kMaxStages), abort_flag, &progress};
     const uint32_t all_bar = bar0 + 8u * (2 * kMaxStages + NB), handed_bar = all_bar + 8, told_bar = handed_bar + 8, ready0 = told_bar + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
     } else if (QUANT && warp >= kQuantWarp0) {
         quantise(p, ring, smem, ready0, scales, walk, off, cum, warp - kQuantWarp0);
     } else if (warp >= kMmaWarp + kIssuers) {
-        hand_over<ACT, W, GATED, ADD>(p, handed_bar, told_bar, &pending, &progress, abort_flag, walk, off, cum);
+        hand_over<ACT, W, GATED, ADD>(p, handed_bar, told_bar, &pending, ring, walk, off, cum);
     } else {
         grid_dep_wait();
         const int quad = warp & 3, half = warp >> 2;
@@ -199,7 +199,6 @@ __global__ void __launch_bounds__(R == 32 ? 512 : 384, 1) matmul_float8_few_kern
             for (int j = 0; j < NR; ++j) acc[j] = 0.0f;
             for (int kb = seg.kb0; kb < seg.kb1; ++kb, ++n) {
                 const int buf = n % NB;
-                if (threadIdx.x == 0) progress = n;
                 const float w = __shfl_sync(0xffffffffu, w0, kb & 31);
                 float f[NX];
                 if (QUANT) {
