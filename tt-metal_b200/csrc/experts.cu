@@ -2,7 +2,8 @@
 //
 // Router. A warp takes a row. An expert's choice value is its logit where that orders the scores (no bias, no sum over a group: the order is then that of exact
 // scores, also where they saturate in 64 bits), else score + bias, first in 32 bits and, for the rows where two values that decide lie closer than that tells, again
-// in 64: the choice is a whole number and has to be that of 64-bit values. Ties go to the lowest index. Bound by instructions, not by the logits' bytes. (All rows in 64 bits: 22 us for 8191 rows of 128.)
+// in 64: the choice is a whole number and has to be that of 64-bit values. Ties go to the lowest index. Bound by instructions, not by the logits' bytes: 8191 rows of 128
+// with bias and 4 of 8 groups, top 6, 19.3 us, 1490 warp instructions a row at 61 % of the issue slots; by logits alone 9.5 us and 780. (All rows in 64 bits: 22 us.)
 //
 // The MLP y[t] = sum_j p[t, j] * down_e( q(act(gate_e x) * (up_e x)) ), e = ids[t, j], runs as
 //   plan      every assignment (t, j) gets a row, sorted by expert and then by t * k + j, with no room between the experts (the matmul's row tiles start at

@@ -14,7 +14,8 @@
 // The blocks that share a tile leave their fp32 sums in scratch and take a ticket; the last one adds them in block order (so results
 // repeat bit for bit) and finishes the rows. No block waits for another. A block's range ends with the first part of a tile, whose other parts are the
 // beginnings of other blocks' ranges: it mostly finds them all there and adds them to its sums in registers.
-// What bounds it (2048 x 8192 x 28672, 477 us in a graph with the quantiser, 2017 TFLOP/s): a block's copies, 48 KB for a unit of 128 x 256 x 128 or 61 B per clock and SM (331 us
+// What bounds it (2048 x 8192 x 28672, 477 us in a graph with the quantiser, 2017 TFLOP/s; 551 us and 1745 TFLOP/s in a loop of seconds, at 1500 MHz under the power
+// limit): a block's copies, 48 KB for a unit of 128 x 256 x 128 or 61 B per clock and SM (331 us
 // by themselves), with the MMAs 398, and the turns of an accumulator, of which two alternate. A tile's results take 3 us to store (fp32 6), and a unit 0.5.
 // Every mbarrier wait is bounded; a wait that runs out raises a status word instead of hanging.
 #include "float8_tiles.cuh"
@@ -334,11 +335,19 @@ static int64_t mean_rows(int64_t rows, int64_t experts) {
     const int64_t hit = rows < experts ? rows : experts;
     return experts ? (rows + hit - 1) / hit : rows;
 }
-// Rows of a tile.
+// Rows of a tile. The experts' MLP in a graph, us, tiles of 32 / 64 / 128 rows:
+//  * 64 experts of 2048 x 1024, chosen evenly: 16 rows each 88 / 93 / 116, 24 rows 93 to 101 / 101 / 117, 32 rows 112 / 105 / 118, 56 rows 141 / 127 / 124, 64 rows 142 / 133 / 126;
+//  * 8 experts of 4096 x 14336, chosen evenly: 24 rows 233 / 240 / 262, 32 rows 238 / 248 / 263, 48 rows 414 / 270 / 270, 56 rows 376 / 280 / 269, 64 rows 351 / 290 / 271.
+// The mean says little where some experts are chosen far more often than others, and the larger tile is then the better one from smaller means on: 8 experts with 24 rows
+// on average and 75 at most 247 / 240 / 208, 32 and 99: 350 / 310 / 268, 56 and 197: 456 / 363 / 256.
 static int rows_per_tile(int64_t rows, int64_t experts) {
     const int64_t mean = mean_rows(rows, experts);
     return mean <= (experts ? 24 : 32) ? 32 : mean <= (experts ? 56 : 64) ? 64 : BM;
 }
+// Up to 8 rows a plain matmul is one launch, quantising its rows itself, and so is the gated one up to 4 rows an expert. That saves a launch where latency counts and costs
+// time with several rows, which every block quantises again for each of its tiles (in a graph, us, itself / by the quantiser's kernel): 1 x 4096 x 1024 9.4 / 9.7, 8 x 4096 x
+// 1024 10.2 / 9.9, 1 x 8192 x 8192 20.1 / 21.2, 8 x 8192 x 8192 22.3 / 21.8, 8 x 4544 x 4672 15.9 / 13.4, 16 x 8192 x 8192 28.6 / 21.5; the experts' MLP, 1 row on 8 of 64 experts of
+// 2048 x 1024 30.0 / 28.4, 4 rows an expert 84.0 / 81.6 (chosen unevenly 62.9 / 54.1), of 8 of 4096 x 14336 218 / 222, 6 rows an expert 221 / 218.
 bool f8_quantises_itself(int64_t rows, int64_t experts) { return mean_rows(rows, experts) <= (experts ? 4 : 8); }
 
 // Weight blocks per tile of a plain matmul. Two make the longer unit of work; which is better goes by the whole rounds over the multiprocessors (us, one / two

@@ -5,7 +5,7 @@
 // warp's lanes and go round by shuffles. Finished sums pass through shared memory, from which whole warps finish row after row: whole lines to memory, and
 // little code, which runs cold once or twice a launch (a thread per row, as the other kernel has it, took 3 to 5 us to store 32 rows of 256 columns).
 // Tiles are shared between blocks as float8_tiles.cuh has it. Bound by the weight's bytes: 1 x 8192 x 28672 40.8 us, 5.8 TB/s; 32 x 8192 x 28672 44.4 us; 32 rows on
-// eight experts of 4096 x 14336 225 us, 6.3 TB/s; small ones by the launch and a hand-over of 2 to 4 us (1 x 4096 x 1024 8.4 us).
+// eight experts of 4096 x 14336 218 to 231 us, 6.1 to 6.5 TB/s; small ones by the launch and a hand-over of 2 to 4 us (1 x 4096 x 1024 8.4 us).
 //
 // Tiles of 8 rows: four more warps quantise the block's rows straight into the operand (QUANT), so that a call is one launch. (For 32 rows the quantising took
 // four times as long as the weights, and a kernel of its own, which this one overlaps, is the better way.)
