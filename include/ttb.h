@@ -241,7 +241,7 @@ int32_t ttb_quantize_float8(const void *src_dev, int32_t src_dtype, int32_t src_
                             int64_t W, int32_t block_rows, void *stream);
 /* out[rows, N] = act( q(a)[rows, K] x w^T + bias ), fp32 accumulation: `a` (bfloat16) is quantised with block_rows 1; w_codes [N, K] and w_scales
  * [ceil(N / 128), ceil(K / 128)] as ttb_quantize_float8 leaves them with block_rows 128 (any positive scales serve). K is a multiple of 16, rows and N are
- * free; tiled tensors have a multiple of 32 rows, and their columns behind N come out as zeros. `bias`: NULL, or bfloat16, the first row of a tiled [32, N]
+ * free (up to 2^24, and up to 2^31 - 1 blocks of 128 activations); tiled tensors have a multiple of 32 rows, and their columns behind N come out as zeros. `bias`: NULL, or bfloat16, the first row of a tiled [32, N]
  * (TTB_MM_BIAS_ROW_MAJOR: [N]). `out`: TTB_BFLOAT16 or TTB_FLOAT32. Flags: TTB_MM_A_ROW_MAJOR, TTB_MM_OUT_ROW_MAJOR, TTB_MM_BIAS_ROW_MAJOR and, as for ttb_matmul,
  * with whose calls a workspace can be shared, TTB_MM_WORKSPACE_ZEROED (else the counters at its head are cleared with a memset) and TTB_MM_WEIGHTS_RESIDENT
  * (not for the call right behind the one that wrote the codes, ttb_quantize_float8 included). The workspace

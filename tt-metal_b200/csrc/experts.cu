@@ -447,6 +447,7 @@ int32_t ttb_experts_mlp_float8(const void *x, const void *ids, const void *weigh
     if (need < 0)
         return fail(TTB_E_INVALID, "%s: between 1 and 2^24 rows times k, hidden and ffn sizes of at most 2^24, 1 to %d experts and k of 1 to %d", who, ttb::kMaxExperts, ttb::kMaxTopK);
     if (hidden % 16 || ffn % 16) return fail(TTB_E_INVALID, "%s: the hidden and ffn sizes must be multiples of 16 (got %lld, %lld)", who, (long long)hidden, (long long)ffn);
+    if (!ttb::f8_blocks_count(rows, hidden)) return fail(TTB_E_UNSUPPORTED, "%s: too many blocks of 128 activations", who);
     for (const void *p : {x, gate_codes, up_codes, down_codes, (const void *)out})
         if (ttb::f8_misaligned(p, 16)) return fail(TTB_E_INVALID, "%s: activations, codes and the result must be 16-byte aligned", who);
     for (const void *p : {ids, weights, gate_scales, up_scales, down_scales})

@@ -449,6 +449,7 @@ int32_t ttb_linear_float8(const void *a, const void *w_codes, const void *w_scal
     const int64_t need = ttb_linear_float8_workspace_bytes(rows, K, N);
     if (need < 0) return fail(TTB_E_INVALID, "ttb_linear_float8: rows, K and N must be between 1 and 2^24");
     if (K % 16) return fail(TTB_E_INVALID, "ttb_linear_float8: K must be a multiple of 16 (got %lld)", (long long)K);
+    if (!ttb::f8_blocks_count(rows, K)) return fail(TTB_E_UNSUPPORTED, "ttb_linear_float8: too many blocks of 128 activations");
     const bool a_rm = flags & TTB_MM_A_ROW_MAJOR, out_rm = flags & TTB_MM_OUT_ROW_MAJOR;
     if ((!a_rm || !out_rm) && rows % 32) return fail(TTB_E_INVALID, "ttb_linear_float8: tiled tensors have a multiple of 32 rows (got %lld)", (long long)rows);
     if (ttb::f8_misaligned(a, 16) || ttb::f8_misaligned(w_codes, 16) || ttb::f8_misaligned(w_scales, 4) || ttb::f8_misaligned(out, out_dtype == TTB_FLOAT32 ? 4 : 2) ||

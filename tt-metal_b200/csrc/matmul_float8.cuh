@@ -69,6 +69,8 @@ int32_t launch_matmul_float8(const F8Matmul &p, cudaStream_t stream);
 // Whether the kernel for these row counts quantises the activations itself.
 bool f8_quantises_itself(int64_t rows, int64_t experts);
 
+// Whether the blocks of 128 values of the rows count in 31 bits, as launch_quantize_operand needs it.
+inline bool f8_blocks_count(int64_t rows, int64_t K) { return rows * f8_blocks(K) <= INT32_MAX; }
 // Quantises [outer, H, K] bfloat16 rows into `out`: row r to row r, or (pos) to the rows pos[r * k + j] >= 0. `early`: lets the next kernel start at once, else
 // when all that came before this one has ended.
 int32_t launch_quantize_operand(const void *a, bool row_major, int64_t outer, int64_t H, int64_t K, const F8Activation &out, const int32_t *pos, int k,
